@@ -230,7 +230,7 @@ def work(case):
 def _e4m3(v):
     """fp64 -> the nearest e4m3 number, ties to even, as fp64 (|v| at most 448 up to rounding)."""
     _, e = torch.frexp(v)                                   # |v| = f 2^e, 1/2 <= f < 1
-    step = torch.ldexp(torch.ones_like(v), e.clamp(min=-5) - 4)
+    step = ((e.long().clamp(min=-5) - 4 + 1023) << 52).view(torch.float64)   # an exact power of two
     return torch.round(v / step) * step
 
 
