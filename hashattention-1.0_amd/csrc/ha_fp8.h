@@ -1,0 +1,42 @@
+// What the 8-bit kernels share: the number format, the block scale and the tile layout of packed weights.
+//
+// e4m3 (OCP: 4 exponent bits, bias 7, 3 mantissa bits, largest 448, no infinities, NaN = 0x7f), one fp32 scale per block of 128
+// consecutive inputs of a row: value = e4m3 number * scale.  For a block with largest magnitude a,
+//     f = max(a, 2^-96),   scale = f / 448 (1 when a = 0),   q = e4m3(y * (448 / f)), round to nearest even.
+// 448 is the largest e4m3 number, so the block's largest element uses the whole range and nothing saturates (448 / f is rounded
+// to fp32, the product lies at most 2 ulp above 448 and rounds to it).  2^-96 keeps 448 / f finite.  An infinity or a NaN
+// in a block makes scale inf or NaN and at least that element NaN: every value of the block, hence every output of the row, is
+// NaN, and no other row is touched.
+#pragma once
+
+#include "ha_common.h"
+
+#define HA_FP8_MAX 448.0f
+#define HA_FP8_FLOOR 0x1p-96f
+
+static inline int ha_fp8_blocks(int K) { return K / HA_FP8_BLOCK + (K % HA_FP8_BLOCK != 0); }
+
+#ifdef __HIPCC__
+
+// four floats -> four e4m3 bytes, the first in the lowest byte
+__device__ __forceinline__ uint32_t ha_fp8x4(float a, float b, float c, float d) {
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
+}
+
+// |y| as bits: ordered as unsigned numbers, finite < infinity < NaN, so a maximum of bits carries a NaN where fmaxf drops it
+__device__ __forceinline__ uint32_t ha_abs_bits(float y) { return __float_as_uint(y) & 0x7FFFFFFFu; }
+
+struct HaFp8Scale {
+    float scale, inv;
+};
+__device__ __forceinline__ HaFp8Scale ha_fp8_scale(uint32_t top_bits) {
+    const float a = __uint_as_float(top_bits);
+    const float f = a < HA_FP8_FLOOR ? HA_FP8_FLOOR : a;  // a NaN compares false and stays
+    HaFp8Scale r;
+    r.inv = HA_FP8_MAX / f;
+    r.scale = top_bits == 0u ? 1.0f : f / HA_FP8_MAX;
+    return r;
+}
+
+#endif  // __HIPCC__

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -146,6 +146,22 @@ def _declare(lib: C.CDLL) -> C.CDLL:
     lib.ha_linear_tiled.argtypes = [vp, i64, vp, vp, i64, i32, vp, i64, i32, i32, i32, vp]
     lib.ha_rmsnorm.restype = i32
     lib.ha_rmsnorm.argtypes = [vp, i64, vp, i32, i32, i32, f32, vp, i64, vp]
+    lib.ha_fp8_row_bytes.restype = i64
+    lib.ha_fp8_row_bytes.argtypes = [i32]
+    lib.ha_quantize_rows_fp8.restype = i32
+    lib.ha_quantize_rows_fp8.argtypes = [vp, i64, i32, i32, i32, vp, i64, vp, i64, vp]
+    lib.ha_rmsnorm_fp8.restype = i32
+    lib.ha_rmsnorm_fp8.argtypes = [vp, i64, vp, i64, vp, i32, i32, i32, f32, vp, i64, vp, i64, vp, i64, vp]
+    lib.ha_swiglu_fp8.restype = i32
+    lib.ha_swiglu_fp8.argtypes = [vp, i64, i32, i32, i32, vp, i64, vp, i64, vp]
+    lib.ha_weight_fp8_bytes.restype = i64
+    lib.ha_weight_fp8_bytes.argtypes = [i32, i32, i32]
+    lib.ha_weight_fp8_scales.restype = i64
+    lib.ha_weight_fp8_scales.argtypes = [i32, i32, i32]
+    lib.ha_pack_weight_fp8.restype = i32
+    lib.ha_pack_weight_fp8.argtypes = [vp, i64, i32, vp, i64, i32, i32, i32, vp, vp, vp]
+    lib.ha_linear_fp8.restype = i32
+    lib.ha_linear_fp8.argtypes = [vp, i64, vp, i64, vp, vp, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp]
     lib.ha_window_partial_bytes.restype = sz
     lib.ha_window_partial_bytes.argtypes = [i32, i32]
     lib.ha_window_partial.restype = i32
@@ -742,4 +758,168 @@ def linear_skinny(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, residual:
     _check(load_library().ha_linear_skinny_fused(_ptr(x), x.stride(0), _ptr(w), w.stride(0), _ptr(residual), res_stride, _ptr(norm_weight),
                                                  float(eps), HA_ACT_SWIGLU if swiglu else HA_ACT_NONE, _ptr(out), out.stride(0), M, N, K,
                                                  _stream(x)), "ha_linear_skinny_fused")
+    return out
+
+
+# ------------------------------------------------------------------------------------------ projections in 8 bits
+
+FP8_BLOCK = 128                 # inputs that share a scale
+HA_FP8_E4M3 = 3
+
+
+class Fp8Weight(NamedTuple):
+    """A weight matrix [N, K] as `linear_fp8` reads it: e4m3 tiles and their scales (`pack_weight_fp8`)."""
+    tiles: torch.Tensor
+    scales: torch.Tensor
+    N: int
+    K: int
+    glu: bool
+
+
+def _same_device(*tensors):
+    """GPU tensors of one device; the launch then runs with that device as the current one."""
+    _require_cuda(*tensors)
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
+def _launch_on(dev, fn, where, *args):
+    """fn(*args, stream) on dev's current stream, with dev as the current device (a kernel launch takes the current one)."""
+    stream = _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        st = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, stream)
+    if st:
+        _check(st, where)
+
+
+def fp8_blocks(k: int) -> int:
+    return -(-k // FP8_BLOCK)
+
+
+def fp8_rows(m: int, k: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Memory for m rows of k elements in 8 bits: (q float8_e4m3fn [m, k rounded up to 128], scales fp32 [m, blocks of 128])."""
+    kb = fp8_blocks(k)
+    return (torch.empty(m, kb * FP8_BLOCK, dtype=torch.float8_e4m3fn, device=device),
+            torch.empty(m, kb, dtype=torch.float32, device=device))
+
+
+def fp8_values(q: torch.Tensor, scales: torch.Tensor, k: int) -> torch.Tensor:
+    """What rows in 8 bits stand for, in fp32 [m, k]."""
+    return (q.float() * scales.repeat_interleave(FP8_BLOCK, dim=1))[:, :k]
+
+
+def _float_rows(t: torch.Tensor, m: int, k: int, what: str, dtype=None) -> None:
+    if t.dim() != 2 or t.shape[0] != m or t.shape[1] != k or (t.stride(1) != 1 and k > 1):
+        raise ValueError(f"{what} must be [{m}, {k}] with contiguous rows, got {tuple(t.shape)} with strides {t.stride()}")
+    if t.dtype not in _DTYPE or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{what} is {t.dtype}" + (f", expected {dtype}" if dtype is not None else ""))
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Stride of the rows; one row (or none) may carry any number there."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _fp8_out(q: torch.Tensor, scales: torch.Tensor, m: int, k: int) -> Tuple[int, int]:
+    kb = fp8_blocks(k)
+    if q.dtype != torch.float8_e4m3fn or q.dim() != 2 or q.shape != (m, kb * FP8_BLOCK) or q.stride(1) != 1:
+        raise ValueError(f"q must be float8_e4m3fn [{m}, {kb * FP8_BLOCK}] with contiguous rows, got {q.dtype} {tuple(q.shape)}")
+    if scales.dtype != torch.float32 or scales.dim() != 2 or scales.shape != (m, kb) or (scales.stride(1) != 1 and kb > 1):
+        raise ValueError(f"scales must be fp32 [{m}, {kb}] with contiguous rows, got {scales.dtype} {tuple(scales.shape)}")
+    return _row_stride(q), _row_stride(scales)
+
+
+def quantize_rows_fp8(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor) -> None:
+    """x [M, K] (fp32, bf16 or fp16) -> rows in 8 bits (`fp8_rows`), one scale per block of 128."""
+    dev = _same_device(x, q, scales)
+    m, k = x.shape
+    _float_rows(x, m, k, "x")
+    q_sm, s_sm = _fp8_out(q, scales, m, k)
+    _launch_on(dev, (_lib or load_library()).ha_quantize_rows_fp8, "ha_quantize_rows_fp8", x.data_ptr(), _row_stride(x), _DTYPE[x.dtype], m, k,
+               q.data_ptr(), q_sm, scales.data_ptr(), s_sm)
+
+
+def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, q: torch.Tensor, scales: torch.Tensor,
+                residual: Optional[torch.Tensor] = None, sum_out: Optional[torch.Tensor] = None) -> None:
+    """h = x (+ residual), rounded to their type; h * rsqrt(mean h^2 + eps) * weight -> rows in 8 bits.  sum_out [M, K]: h, for the
+    layer's next addition; it may be x or residual itself."""
+    dev = _same_device(x, weight, q, scales, residual, sum_out)
+    m, k = x.shape
+    _float_rows(x, m, k, "x")
+    if weight.dtype != x.dtype or weight.shape != (k,) or not weight.is_contiguous():
+        raise ValueError(f"weight must be {x.dtype} [{k}], got {weight.dtype} {tuple(weight.shape)}")
+    if residual is not None:
+        _float_rows(residual, m, k, "residual", x.dtype)
+    if sum_out is not None:
+        _float_rows(sum_out, m, k, "sum_out", x.dtype)
+    q_sm, s_sm = _fp8_out(q, scales, m, k)
+    _launch_on(dev, (_lib or load_library()).ha_rmsnorm_fp8, "ha_rmsnorm_fp8", x.data_ptr(), _row_stride(x), _ptr(residual),
+               0 if residual is None else _row_stride(residual), weight.data_ptr(), _DTYPE[x.dtype], m, k, float(eps), _ptr(sum_out),
+               0 if sum_out is None else _row_stride(sum_out), q.data_ptr(), q_sm, scales.data_ptr(), s_sm)
+
+
+def swiglu_fp8(gate_up: torch.Tensor, q: torch.Tensor, scales: torch.Tensor) -> None:
+    """gate_up [M, 2 F] (gate | up) -> silu(gate) * up as rows of F in 8 bits."""
+    dev = _same_device(gate_up, q, scales)
+    m, k2 = gate_up.shape
+    _float_rows(gate_up, m, k2, "gate_up")
+    if k2 % 2:
+        raise ValueError(f"gate_up must hold an even number of columns, got {k2}")
+    q_sm, s_sm = _fp8_out(q, scales, m, k2 // 2)
+    _launch_on(dev, (_lib or load_library()).ha_swiglu_fp8, "ha_swiglu_fp8", gate_up.data_ptr(), _row_stride(gate_up), _DTYPE[gate_up.dtype], m,
+               k2 // 2, q.data_ptr(), q_sm, scales.data_ptr(), s_sm)
+
+
+def pack_weight_fp8(w: torch.Tensor, scales: Optional[torch.Tensor] = None, glu: bool = False) -> Fp8Weight:
+    """The 8-bit copy of a weight matrix w [N, K] that `linear_fp8` reads.  w fp32, bf16 or fp16: quantised here, one scale per block of
+    128 x 128.  w float8_e4m3fn with scales fp32 [ceil(N / 128), ceil(K / 128)]: taken over as they are.  glu: w = [gate rows; up
+    rows], each matrix with blocks of its own (scales: those of gate, then those of up)."""
+    dev = _same_device(w, scales)
+    if w.dim() != 2 or w.numel() == 0 or (w.stride(1) != 1 and w.shape[1] > 1):
+        raise ValueError(f"w must be [N, K] with contiguous rows, got {tuple(w.shape)} with strides {w.stride()}")
+    n, k = w.shape
+    if glu and n % 2:
+        raise ValueError(f"gate and up rows need an even number of weight rows, got {n}")
+    if w.dtype == torch.float8_e4m3fn:
+        blocks = (2 * fp8_blocks(n // 2) if glu else fp8_blocks(n), fp8_blocks(k))
+        if scales is None or scales.dtype != torch.float32 or scales.shape != blocks or (scales.stride(1) != 1 and blocks[1] > 1):
+            raise ValueError(f"weights in e4m3 come with fp32 scales {list(blocks)}")
+        dtype = HA_FP8_E4M3
+    elif w.dtype in _DTYPE:
+        if scales is not None:
+            raise ValueError(f"scales belong to weights in e4m3, w is {w.dtype}")
+        dtype = _DTYPE[w.dtype]
+    else:
+        raise ValueError(f"w is {w.dtype}: fp32, bf16, fp16 or float8_e4m3fn")
+    lib = load_library()
+    out = Fp8Weight(torch.empty(lib.ha_weight_fp8_bytes(n, k, int(glu)), dtype=torch.uint8, device=dev),
+                    torch.empty(lib.ha_weight_fp8_scales(n, k, int(glu)), dtype=torch.float32, device=dev), n, k, bool(glu))
+    _launch_on(dev, lib.ha_pack_weight_fp8, "ha_pack_weight_fp8", w.data_ptr(), _row_stride(w), dtype, _ptr(scales),
+               0 if scales is None else _row_stride(scales), n, k, int(glu), out.tiles.data_ptr(), out.scales.data_ptr())
+    return out
+
+
+def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: torch.Tensor, residual: Optional[torch.Tensor] = None,
+               swiglu: bool = False) -> torch.Tensor:
+    """out [M, N] = rows in 8 bits (q, scales) . W^T (+ residual), or [M, N / 2] = silu(gate) * up with swiglu (weights packed with
+    glu); out fp32, bf16 or fp16, rounded once.  residual may be out itself."""
+    dev = _same_device(q, scales, weight.tiles, weight.scales, out, residual)
+    m, n = q.shape[0], weight.N
+    q_sm, s_sm = _fp8_out(q, scales, m, weight.K)
+    if weight.glu != swiglu:
+        raise ValueError("swiglu takes weights packed with glu, and nothing else does")
+    _float_rows(out, m, n // 2 if swiglu else n, "out")
+    if residual is not None:
+        if swiglu:
+            raise ValueError("SwiGLU takes no residual")
+        _float_rows(residual, m, n, "residual", out.dtype)
+    _launch_on(dev, (_lib or load_library()).ha_linear_fp8, "ha_linear_fp8", q.data_ptr(), q_sm, scales.data_ptr(), s_sm, weight.tiles.data_ptr(),
+               weight.scales.data_ptr(), _ptr(residual), 0 if residual is None else _row_stride(residual),
+               HA_ACT_SWIGLU if swiglu else HA_ACT_NONE, out.data_ptr(), _row_stride(out), _DTYPE[out.dtype], m, n, weight.K)
     return out

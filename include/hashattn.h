@@ -501,6 +501,54 @@ int ha_pack_weight_tiles(const void *w, int64_t w_stride_n, int N, int K, int gl
 int ha_linear_tiled(const void *x, int64_t x_stride_m, const void *tiles, const void *residual, int64_t residual_stride_m,
                     int act, void *out, int64_t out_stride_m, int M, int N, int K, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Projections in 8 bits.  Rows of x and weights are e4m3 numbers (OCP: 4 exponent bits, 3 mantissa bits, largest 448, no
+ * infinities) with one fp32 scale per block of HA_FP8_BLOCK = 128 inputs: per row of x, and per 128 x 128 block of a weight
+ * matrix (the last blocks may be narrower).  A value is its number times its scale.  Half the bytes of bf16 weights in a decode
+ * step, twice the matrix cores' rate on a prompt.  No counterpart in the reference, whose projections are bf16 nn.Linear.
+ *
+ * Rows in 8 bits: q uint8 [M, ha_fp8_row_bytes(K)] (K rounded up to whole blocks, zero beyond K), rows 16-byte aligned,
+ * q_stride_m in bytes; scales fp32 [M, ceil(K / 128)].  Scale of a block with largest magnitude a: max(a, 2^-96) / 448, and 1 for
+ * a block of zeros.  A block that holds an infinity or a NaN comes back as NaN, and with it the row's outputs; other rows are not
+ * touched.  M = 0 is no work and no error; what lies behind the last row and behind a row's last block is left as it was.
+ *   ha_quantize_rows_fp8   x [M, K] of dtype
+ *   ha_rmsnorm_fp8         h = x (+ residual), rounded to dtype; y = h * rsqrt(mean_k h^2 + eps) * weight in fp32 and straight to
+ *                          8 bits.  sum_out (may be NULL): h [M, K], which the layer's next addition takes; it may be x's or the
+ *                          residual's own memory (same pointer and stride), any other overlap is not supported.  K <= 65536
+ *   ha_swiglu_fp8          gate_up [M, 2 F] (gate | up): silu(gate) * up in fp32 and straight to 8 bits, rows of F
+ * Any alignment of x, weight, residual and sum_out to their elements is taken; rows on 16-byte boundaries are read faster.
+ *
+ * Weights are packed once, in the order the matrix instruction reads them:
+ *   ha_weight_fp8_bytes / _scales   sizes of the packed copy of a [N, K] matrix: bytes of `tiles`, floats of `tile_scales` (0 for
+ *                                   a bad shape)
+ *   ha_pack_weight_fp8              w [N, K] of dtype, w_scales NULL: quantised here.  dtype HA_FP8_E4M3 with w_scales fp32
+ *                                   [ceil(N / 128), ceil(K / 128)]: taken over as they are.  glu = 1: w is [F gate rows; F up
+ *                                   rows] (N = 2 F), each matrix with blocks of its own: w_scales then holds gate's rows of
+ *                                   ceil(F / 128) blocks, then up's
+ *
+ * ha_linear_fp8: out [M, N] = x . W^T (+ residual [M, N] of out_dtype), or with act = HA_ACT_SWIGLU (weights packed with glu = 1)
+ * out [M, N / 2] = silu(gate) * up.  Products exact, sums in fp32, ONE rounding to out_dtype at the end (residual and SwiGLU before
+ * it).  Any M, N, K; `residual` may be `out` itself.  Which kernel runs depends on the sizes alone; a row's outputs do not
+ * depend on the other rows.
+ */
+#define HA_FP8_BLOCK 128
+#define HA_FP8_E4M3 3 /* dtype code of ha_pack_weight_fp8 only */
+int64_t ha_fp8_row_bytes(int K);
+int ha_quantize_rows_fp8(const void *x, int64_t x_stride_m, int dtype, int M, int K, void *q, int64_t q_stride_m, float *scales,
+                         int64_t scales_stride_m, void *stream);
+int ha_rmsnorm_fp8(const void *x, int64_t x_stride_m, const void *residual, int64_t residual_stride_m, const void *weight, int dtype, int M,
+                   int K, float eps, void *sum_out, int64_t sum_stride_m, void *q, int64_t q_stride_m, float *scales,
+                   int64_t scales_stride_m, void *stream);
+int ha_swiglu_fp8(const void *gate_up, int64_t gate_up_stride_m, int dtype, int M, int F, void *q, int64_t q_stride_m, float *scales,
+                  int64_t scales_stride_m, void *stream);
+int64_t ha_weight_fp8_bytes(int N, int K, int glu);
+int64_t ha_weight_fp8_scales(int N, int K, int glu);
+int ha_pack_weight_fp8(const void *w, int64_t w_stride_n, int dtype, const float *w_scales, int64_t w_scales_stride_n, int N, int K, int glu,
+                       void *tiles, float *tile_scales, void *stream);
+int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, int64_t x_scales_stride_m, const void *tiles,
+                  const float *tile_scales, const void *residual, int64_t residual_stride_m, int act, void *out, int64_t out_stride_m,
+                  int out_dtype, int M, int N, int K, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
