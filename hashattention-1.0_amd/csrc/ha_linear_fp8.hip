@@ -16,6 +16,7 @@
 
 namespace {
 
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -124,7 +125,48 @@ struct Epilogue {
     void *out;
     int64_t out_sm;
     int out_dtype;
+    bool wide, wide8;  // four neighbouring columns of out and residual, eight of out are one aligned access
 };
+
+// y += residual[m, n .. min(n + 4, cols))
+__device__ __forceinline__ void add_residual(const Epilogue &ep, int64_t m, int n, int cols, f32x4 &y) {
+    if (ep.wide && n + 4 <= cols) {
+        if (ep.out_dtype == HA_F32) {
+            y += *reinterpret_cast<const f32x4 *>((const float *)ep.res + m * ep.res_sm + n);
+        } else {
+            const uint2 b = *reinterpret_cast<const uint2 *>((const uint16_t *)ep.res + m * ep.res_sm + n);
+            const uint32_t w[4] = {b.x & 0xFFFFu, b.x >> 16, b.y & 0xFFFFu, b.y >> 16};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                y[i] += ep.out_dtype == HA_BF16 ? __uint_as_float(w[i] << 16) : __half2float(__ushort_as_half((unsigned short)w[i]));
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < cols) y[i] += ha_load_elem(ep.res, m * ep.res_sm + n + i, ep.out_dtype);
+}
+
+// four results as 16-bit numbers
+__device__ __forceinline__ uint2 narrow4(const f32x4 &y, int dtype) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = dtype == HA_BF16 ? ha_f32_to_bf16_bits(y[i]) : (uint32_t)__half_as_ushort(__float2half(y[i]));
+    return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+}
+
+// fp32 out[m, n .. min(n + 4, cols)) = y (+ residual)
+__device__ __forceinline__ void store4(const Epilogue &ep, int64_t m, int n, int cols, f32x4 y) {
+    if (ep.res) add_residual(ep, m, n, cols, y);
+    float *o = (float *)ep.out + m * ep.out_sm + n;
+    if (ep.wide && n + 4 <= cols) {
+        *reinterpret_cast<f32x4 *>(o) = y;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < cols) o[i] = y[i];
+}
 
 // The simple form, for any size: one tile of 16 weight rows and 16 MT rows of x per workgroup, the blocks of K dealt out to its
 // waves, their sums joined through LDS.
@@ -190,6 +232,274 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_kernel(const uint8_t *_
     }
 }
 
+// ---- many rows: tiles of BN weight rows x BM rows of x per workgroup, staged through LDS
+//
+// WN x WM waves of TN x TM operand tiles each (16 weight rows, 16 rows of x).  Everything a block of 128 inputs needs travels
+// from memory straight to LDS (one KiB per request and wave).  Weights lie there in the order the matrix instruction takes
+// them, lane l's 16 bytes at l * 16.  Rows of x arrive as whole 128-byte lines, eight to a request; the 16-byte chunk c of row r
+// sits in place c ^ (r & 7) of its line - each lane asks for the chunk that belongs in its place - so that the eight lanes that an
+// LDS read serves at a time, same chunk of eight rows, meet eight different bank groups.
+//
+// Two buffers, each in two parts: x with the first half of every wave's weight tiles, and the second half.  A part is requested
+// as soon as all waves have read the part of two blocks before out of its place, half a block's time after the other: between
+// its request and its use lie one and a half blocks' time, and three quarters of the buffers are always on their way.
+// EXACT: bf16 matrix instructions on widened operands; otherwise the 8-bit ones (see the top of this file).
+template <bool EXACT>
+struct TileOperand;
+template <>
+struct TileOperand<false> {
+    i32x8 v;
+    __device__ __forceinline__ void load(const uint8_t *first, const uint8_t *second) {
+        const uint4 a = *reinterpret_cast<const uint4 *>(first), b = *reinterpret_cast<const uint4 *>(second);
+        v = i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+    }
+    // constant zero scale operands select the instruction without block exponents
+    __device__ static __forceinline__ f32x4 product(const TileOperand &w, const TileOperand &x) {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+    }
+};
+template <>
+struct TileOperand<true> {
+    Wide v;
+    __device__ __forceinline__ void load(const uint8_t *first, const uint8_t *second) {
+        v = widen(*reinterpret_cast<const uint4 *>(first), *reinterpret_cast<const uint4 *>(second));
+    }
+    __device__ static __forceinline__ f32x4 product(const TileOperand &w, const TileOperand &x) { return block_sum(w.v, x.v); }
+};
+
+// Requests from memory straight to LDS: lane l's 16 (4) bytes from base + offset + from, and i * kStep more for the i-th of a call,
+// land at lds + l * 16 (l * 4) + i * kStep; `from` and lds are uniform over the wave.  A buffer resource takes its base from four
+// scalar registers and `from` from a fifth, so that a request costs no address arithmetic; the instruction's own offset counts
+// for both sides, which is why targets of one call lie kStep apart.
+// Inline assembly, because the compiler would wait for all of them in front of every LDS read it cannot tell from their target;
+// the waits are written by hand (requests_arrived).  M0 holds the LDS address; nothing else in the kernel uses M0.
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4 resource(const void *base) {  // uniform base; every access of this file is in bounds by itself
+    const uint64_t b = (uint64_t)base;
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32)),
+                 0xFFFFFFFFu, 0x00020000u};
+}
+__device__ __forceinline__ void request16x2(u32x4 res, uint32_t offset, uint32_t from, uint32_t lds) {  // kStep 1024
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds\n\t"
+                 "buffer_load_dwordx4 %0, %1, %3 offen offset:1024 lds"
+                 ::"v"(offset), "s"(res), "s"(lds), "s"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void request16x4(u32x4 res, const uint32_t (&offset)[4], uint32_t from, uint32_t lds) {  // kStep 1024
+    asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %4, %6 offen lds\n\t"
+                 "buffer_load_dwordx4 %1, %4, %6 offen offset:1024 lds\n\t"
+                 "buffer_load_dwordx4 %2, %4, %6 offen offset:2048 lds\n\t"
+                 "buffer_load_dwordx4 %3, %4, %6 offen offset:3072 lds"
+                 ::"v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3]), "s"(res), "s"(lds), "s"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void request4(u32x4 res, uint32_t offset, uint32_t from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %3 offen lds" ::"v"(offset), "s"(res), "s"(lds), "s"(from) : "memory");
+}
+// Waits until at most `younger` of the wave's requests are outstanding (they arrive in the order they were made) and every wave
+// has come here; all LDS reads of the wave have arrived too.
+template <int YOUNGER>
+__device__ __forceinline__ void requests_arrived() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(YOUNGER) : "memory");
+    __syncthreads();
+}
+
+template <int WN, int WM, int TN, int TM, int AHEAD, bool EXACT, bool GLU>
+__global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uint8_t *__restrict__ x, int64_t x_sm,
+                                                                       const float *__restrict__ xs, int64_t xs_sm,
+                                                                       const uint8_t *__restrict__ tiles, const float *__restrict__ ws,
+                                                                       Epilogue ep, int M, int N, int kb_count, int n_tiles, int tiles_n,
+                                                                       int tiles_m, int per_xcd) {
+    constexpr int NW = WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, TH = TN / 2;
+    constexpr int kWBytes = BN * HA_FP8_BLOCK, kXBytes = BM * HA_FP8_BLOCK, kBuffer = kWBytes + kXBytes;
+    constexpr int kHalfPieces = kWBytes / 2048 / NW, kXPieces = kXBytes / 1024 / NW;  // requests per wave: half of the weights, x
+    constexpr int kFirst = kXPieces + kHalfPieces + 2, kSecond = kHalfPieces;          // requests per wave and part (two for the scales)
+    static_assert(kWBytes % (2048 * NW) == 0 && kXBytes % (1024 * NW) == 0 && BM <= 64 * NW && BM % 64 == 0, "pieces deal out evenly");
+    static_assert(TN % 2 == 0 && 16 * TN <= HA_FP8_BLOCK, "one weight scale per wave, half and block");
+    __shared__ __attribute__((aligned(1024))) uint8_t s_buf[2][kBuffer];
+    __shared__ float s_xs[2][BM], s_ws[2][NW * 64];
+    // Workgroups go to the XCDs in turn: XCD j takes a run of tiles, four tiles of x wide and then along N, so that the 32 CUs
+    // that share an L2 work on a compact block of the result.
+    const int linear = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if (linear >= tiles_n * tiles_m) return;
+    const int band = linear / (4 * tiles_n), in_band = linear - band * 4 * tiles_n, rows_in_band = min(4, tiles_m - 4 * band);
+    const int bm = 4 * band + in_band % rows_in_band, bn = in_band / rows_in_band;
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
+    const int m0 = bm * BM, nt0 = bn * (BN / 16);
+
+    // rows and tiles beyond the matrices are read as their last ones; what they give is not stored
+    static_assert(kXPieces == 4 && kHalfPieces == 2, "requests are made by four and by two");
+    const u32x4 x_res = resource(x + (int64_t)m0 * x_sm - 4096), xs_res = resource(xs + (int64_t)m0 * xs_sm);
+    const u32x4 w_res = resource(tiles + (int64_t)nt0 * kb_count * kTileBytes);
+    // all tiles of a wave lie in one block of 128 weight rows (glu: one of gate and one of up): one scale per lane and block of K
+    const u32x4 ws_res = resource(ws + (int64_t)min(nt0 + wn * TN, n_tiles - 1) * kb_count * 2);
+    uint32_t x_off[4], w_off[2], w_at[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // 4096 - 1024 i: what the resource's base and the request's own offset take away and add
+        const int row = (wave * 4 + i) * 8 + (lane >> 3);
+        x_off[i] = (uint32_t)min(row, M - 1 - m0) * (uint32_t)x_sm + ((lane ^ row) & 7) * 16 + 4096 - 1024 * i;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // the wave's tile of each half
+        const int tile = wave / TH * TN + h * TH + wave % TH;
+        w_at[h] = tile * kTileBytes;
+        w_off[h] = (uint32_t)min(tile, n_tiles - 1 - nt0) * (uint32_t)kb_count * kTileBytes + lane * 16;
+    }
+    const uint32_t xs_off = (uint32_t)min((wave % (BM / 64)) * 64 + lane, M - 1 - m0) * (uint32_t)xs_sm * 4u, ws_off = (g >> 1) * 4u;
+    const uint32_t lds_buf = (uint32_t)(uintptr_t)&s_buf[0][0], lds_xs = (uint32_t)(uintptr_t)&s_xs[0][0], lds_ws = (uint32_t)(uintptr_t)&s_ws[0][0];
+    // kb: the place; from min(kb, last), so that the loop's requests (hence its waits) are the same in every turn
+    auto request_half = [&](int kb, int h) {
+        request16x2(w_res, w_off[h], min(kb, kb_count - 1) * kTileBytes, lds_buf + (kb & 1) * kBuffer + w_at[h]);
+    };
+    auto request_x = [&](int kb) {
+        request16x4(x_res, x_off, min(kb, kb_count - 1) * HA_FP8_BLOCK, lds_buf + (kb & 1) * kBuffer + kWBytes + wave * 4096);
+    };
+    auto request_scales = [&](int kb) {
+        request4(xs_res, xs_off, min(kb, kb_count - 1) * 4, lds_xs + ((kb & 1) * BM + wave % (BM / 64) * 64) * 4);
+        request4(ws_res, ws_off, min(kb, kb_count - 1) * 8, lds_ws + ((kb & 1) * NW + wave) * 256);
+    };
+
+    f32x4 acc[TN][TM];
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+        for (int u = 0; u < TM; ++u) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // LDS addresses of a wave's operands within a buffer
+    const uint32_t x_first = kWBytes + (wm * TM * 16 + r) * HA_FP8_BLOCK + ((g ^ r) & 7) * 16, x_second = x_first ^ 64;
+    const uint32_t w_first = wn * TN * kTileBytes + lane * 16;
+    constexpr int kAhead = AHEAD, kRing = kAhead + 1;  // tiles of weights read ahead of the one in use
+    TileOperand<EXACT> xo[TM], wo[kRing];
+    f32x4 part[2][TM];
+    float s[TM], s_next[TM + 1];  // of the next block as they lie in LDS: rows of x, weights
+    auto load_row = [&](int kb, int u) {
+        const uint8_t *b = &s_buf[0][0] + (kb & 1) * kBuffer + u * kTileBytes;
+        xo[u].load(b + x_first, b + x_second);
+    };
+    auto load_scales = [&](int kb) {
+        s_next[TM] = s_ws[kb & 1][wave * 64 + lane];
+#pragma unroll
+        for (int u = 0; u < TM; ++u) s_next[u] = s_xs[kb & 1][(wm * TM + u) * 16 + r];
+    };
+    auto load_weights = [&](TileOperand<EXACT> &w, int kb, int t) {
+        const uint8_t *b = &s_buf[0][0] + (kb & 1) * kBuffer + w_first + t * kTileBytes;
+        w.load(b, b + 1024);
+    };
+    static_assert(TN % kRing == 0 && kAhead < TH, "a block ends on the operand register it began with; its halves are further apart");
+    // the order of requests: of every block x, scales, first half, then the second half
+    request_x(0);
+    request_scales(0);
+    request_half(0, 0);
+    request_half(0, 1);
+    request_x(1);
+    request_scales(1);
+    request_half(1, 0);
+    request_half(1, 1);
+    requests_arrived<kFirst + 2 * kSecond>();
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) load_weights(wo[t], 0, t);
+#pragma unroll
+    for (int u = 0; u < TM; ++u) load_row(0, u);
+    load_scales(0);
+    // One block of 128 inputs per turn: TN x TM matrix instructions, the multiply-adds of a tile under those of the next one, weights
+    // read from LDS kAhead tiles ahead, a row of the next block's x as soon as its last instruction is issued.
+    for (int kb = 0; kb < kb_count; ++kb) {
+#pragma unroll
+        for (int u = 0; u < TM; ++u) s[u] = s_next[u] * s_next[TM];
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+            if (t == TH - kAhead) {
+                // every wave has x and the first half of this block's weights in registers: the block after next takes their
+                // place.  Arrived: the second half of this block.
+                requests_arrived<kFirst + kSecond>();
+                request_x(kb + 2);
+            }
+            if (t == TH - kAhead + 1) {
+                request_scales(kb + 2);
+                request_half(kb + 2, 0);
+            }
+            if (t == TN - kAhead) {
+                // every wave has the second half in registers too.  Arrived: x and the first half of the next block.
+                requests_arrived<kFirst + kSecond>();
+                request_half(kb + 2, 1);
+            }
+            if (t + kAhead < TN) load_weights(wo[(t + kAhead) % kRing], kb, t + kAhead);
+            else load_weights(wo[(t + kAhead) % kRing], kb + 1, t + kAhead - TN);
+            if (t == TN - 1) load_scales(kb + 1);
+#pragma unroll
+            for (int u = 0; u < TM; ++u) {
+                part[t & 1][u] = TileOperand<EXACT>::product(wo[t % kRing], xo[u]);
+                if (t == TN - 1) load_row(kb + 1, u);
+                if (t > 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[t - 1][u][i] = fmaf(part[(t - 1) & 1][u][i], s[u], acc[t - 1][u][i]);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // as written: the compiler would hoist the LDS reads of all tiles and spill
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < TM; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[TN - 1][u][i] = fmaf(part[(TN - 1) & 1][u][i], s[u], acc[TN - 1][u][i]);
+    }
+    requests_arrived<0>();
+
+    // acc[t][u][i]: weight row 4 g + i of tile t, row 16 u + r of x
+    constexpr int BO = GLU ? BN / 2 : BN;  // columns of out per workgroup
+    const int n_out = GLU ? N / 2 : N, n0 = bn * BO;
+    auto each = [&](auto put) {
+#pragma unroll
+        for (int u = 0; u < TM; ++u)
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                f32x4 y = acc[t][u];
+                int col = (wn * TN + t) * 16 + 4 * g;
+                if constexpr (GLU) {  // gate in lanes 0 - 31, up in lanes 32 - 63
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float up = __shfl_xor(acc[t][u][i], 32);
+                        y[i] = acc[t][u][i] / (1.0f + expf(-acc[t][u][i])) * up;
+                    }
+                    col = (wn * TN + t) * 8 + 4 * g;
+                    if (g >= 2) continue;
+                }
+                put((wm * TM + u) * 16 + r, col, y);
+            }
+    };
+    if (ep.out_dtype == HA_F32) {
+        each([&](int row, int col, f32x4 y) {
+            if (m0 + row < M && n0 + col < n_out) store4(ep, m0 + row, n0 + col, n_out, y);
+        });
+        return;
+    }
+    // 16-bit results leave through LDS, so that whole lines are written: a wave's registers hold four columns of sixteen rows.
+    // The 16-byte piece c of row m sits in place c ^ (m & 15), within the row's power of two of pieces: the sixteen rows a wave
+    // stores at a time meet different banks.
+    uint8_t *tile = &s_buf[0][0];
+    static_assert(BM * BO * 2 <= 2 * kBuffer, "the result fits where the operands were");
+    constexpr int kRowPieces = BO / 8, kTurn = (kRowPieces < 16 ? kRowPieces : 16) - 1;
+    static_assert((kRowPieces & (kRowPieces - 1)) == 0, "pieces turn within their row");
+    each([&](int row, int col, f32x4 y) {
+        if (ep.res) add_residual(ep, m0 + row, n0 + col, (m0 + row < M) ? n_out : 0, y);
+        *reinterpret_cast<uint2 *>(tile + row * (BO * 2) + (((col >> 3) ^ (row & kTurn)) * 16) + (col & 4) * 2) = narrow4(y, ep.out_dtype);
+    });
+    __syncthreads();
+    for (int i = tid; i < BM * kRowPieces; i += NW * 64) {
+        const int row = i / kRowPieces, c = i % kRowPieces, n = n0 + c * 8;
+        if (m0 + row >= M || n >= n_out) continue;
+        const uint4 v = *reinterpret_cast<const uint4 *>(tile + row * (BO * 2) + ((c ^ (row & kTurn)) * 16));
+        uint16_t *o = (uint16_t *)ep.out + (int64_t)(m0 + row) * ep.out_sm + n;
+        if (ep.wide8 && n + 8 <= n_out) {
+            *reinterpret_cast<uint4 *>(o) = v;
+        } else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (n + k < n_out) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+        }
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -246,7 +556,29 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
                "pointers are not aligned to their elements");
     int st = ha_require_device();
     if (st || M == 0) return st;
-    const Epilogue ep = {residual, residual_stride_m, out, out_stride_m, out_dtype};
+    const bool wide = ha_aligned(out, 4 * es) && out_stride_m % 4 == 0 && (!residual || (ha_aligned(residual, 4 * es) && residual_stride_m % 4 == 0));
+    const Epilogue ep = {residual, residual_stride_m, out, out_stride_m, out_dtype, wide, ha_aligned(out, 8 * es) && out_stride_m % 8 == 0};
+    if (M > 128 && 256 * (xq_stride_m + x_scales_stride_m * 4) < (1LL << 31) && (int64_t)p.kb * kTileBytes * 16 < (1LL << 31)) {
+        const bool exact = out_dtype == HA_F32;
+        const int64_t big = ((p.n_tiles + 15LL) / 16) * ((M + 255LL) / 256);
+        const bool use_big = !exact && big >= 200;
+        const int tiles_n = use_big ? (p.n_tiles + 15) / 16 : (p.n_tiles + 7) / 8, tiles_m = use_big ? (M + 255) / 256 : (M + 127) / 128;
+        const int64_t total = (int64_t)tiles_n * tiles_m, per_xcd = (total + 7) / 8;
+        HA_REQUIRE(total <= 2147483647LL / 8, HA_ERR_BAD_SHAPE, "too many tiles for one launch");
+#define HA_TILED(WN_, WM_, TN_, TM_, A_, E_, G_)                                                                                             \
+    hipLaunchKernelGGL((linear_fp8_tiled_kernel<WN_, WM_, TN_, TM_, A_, E_, G_>), dim3((unsigned)(8 * per_xcd)), dim3(WN_ * WM_ * 64), 0,    \
+                       (hipStream_t)stream, (const uint8_t *)xq, xq_stride_m, x_scales, x_scales_stride_m, (const uint8_t *)tiles,       \
+                       tile_scales, ep, M, N, p.kb, p.n_tiles, tiles_n, tiles_m, (int)per_xcd)
+        if (exact && act) HA_TILED(2, 2, 4, 4, 1, true, true);
+        else if (exact) HA_TILED(2, 2, 4, 4, 1, true, false);
+        else if (use_big && act) HA_TILED(2, 4, 8, 4, 3, false, true);
+        else if (use_big) HA_TILED(2, 4, 8, 4, 3, false, false);
+        else if (act) HA_TILED(2, 2, 4, 4, 1, false, true);
+        else HA_TILED(2, 2, 4, 4, 1, false, false);
+#undef HA_TILED
+        HA_CHECK_LAUNCH("linear_fp8_tiled_kernel");
+        return HA_OK;
+    }
     const int MT = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     const int64_t grid = (int64_t)p.n_tiles * ((M + 16LL * MT - 1) / (16 * MT));
     HA_REQUIRE(grid <= 2147483647LL, HA_ERR_BAD_SHAPE, "too many tiles for one launch");
