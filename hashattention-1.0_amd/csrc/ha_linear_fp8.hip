@@ -8,7 +8,9 @@
 // products at a time and drop what lies more than 13 bits below the largest of the eight (measured: 2^3 beside 2^16 is kept,
 // 2^2 is lost, wherever the two sit within eight inputs; further apart the sum is fp32).  On normally distributed numbers that
 // is 1.5e-5 of the result, 1e-4 where magnitudes spread widely.  e4m3 numbers are exact in bf16 and v_mfma_f32_16x16x32_bf16
-// keeps its sums in fp32 (1.2e-8 on the same numbers), at half the 8-bit rate plus one conversion per two numbers.
+// keeps its sums in fp32 (1.2e-8 on the same numbers), at half the 8-bit rate plus one conversion per two numbers.  So: fp32
+// results and up to 16 rows, where the stream of weights is the bound and the conversions cost nothing, run on the bf16
+// instruction; 16-bit results of more rows, whose own rounding (2^-9 or 2^-12 of the value) is a hundred times that, on the 8-bit one.
 //
 //   ha_weight_fp8_bytes / ha_weight_fp8_scales / ha_pack_weight_fp8   the packed weights
 //   ha_linear_fp8                                                     the product, residual or SwiGLU behind
@@ -119,6 +121,28 @@ __device__ __forceinline__ f32x4 block_sum(const Wide &w, const Wide &x) {
     return c;
 }
 
+// An operand of a block of 128 inputs, made of a lane's two pieces.  EXACT: bf16 matrix instructions on widened numbers; otherwise the
+// 8-bit one (see the top of this file).
+template <bool EXACT>
+struct Operand;
+template <>
+struct Operand<false> {
+    i32x8 v;
+    __device__ __forceinline__ void take(const uint4 &a, const uint4 &b) {
+        v = i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+    }
+    // constant zero scale operands select the instruction without block exponents
+    __device__ static __forceinline__ f32x4 product(const Operand &w, const Operand &x) {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+    }
+};
+template <>
+struct Operand<true> {
+    Wide v;
+    __device__ __forceinline__ void take(const uint4 &a, const uint4 &b) { v = widen(a, b); }
+    __device__ static __forceinline__ f32x4 product(const Operand &w, const Operand &x) { return block_sum(w.v, x.v); }
+};
+
 struct Epilogue {
     const void *res;
     int64_t res_sm;
@@ -168,46 +192,10 @@ __device__ __forceinline__ void store4(const Epilogue &ep, int64_t m, int n, int
         if (n + i < cols) o[i] = y[i];
 }
 
-// The simple form, for any size: one tile of 16 weight rows and 16 MT rows of x per workgroup, the blocks of K dealt out to its
-// waves, their sums joined through LDS.
+// The waves' sums of tile nt (s_c[wave][weight row][row of x]) joined, finished and stored by the whole workgroup.
 template <int NWAVE, int MT, bool GLU>
-__global__ __launch_bounds__(NWAVE * 64) void linear_fp8_kernel(const uint8_t *__restrict__ x, int64_t x_sm, const float *__restrict__ xs,
-                                                                int64_t xs_sm, const uint8_t *__restrict__ tiles,
-                                                                const float *__restrict__ ws, Epilogue ep, int M, int N, int kb_count,
-                                                                int n_tiles) {
-    __shared__ float s_c[NWAVE][16][16 * MT + 1];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, g = lane >> 4;
-    const int nt = (int)(blockIdx.x % (unsigned)n_tiles), m0 = (int)(blockIdx.x / (unsigned)n_tiles) * 16 * MT;
-    const uint8_t *tp = tiles + (int64_t)nt * kb_count * kTileBytes + lane * 16;
-    const float *wsp = ws + (int64_t)nt * kb_count * 2 + (g >> 1);
-    f32x4 acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < kb_count; kb += NWAVE) {
-        const uint4 *wt = reinterpret_cast<const uint4 *>(tp + (int64_t)kb * kTileBytes);
-        const Wide wv = widen(wt[0], wt[64]);
-        const float w_scale = wsp[2 * kb];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const int m = m0 + 16 * t + r;
-            uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
-            float s = 0.f;
-            if (m < M) {
-                const uint4 *xp = reinterpret_cast<const uint4 *>(x + m * x_sm + kb * HA_FP8_BLOCK + g * 16);
-                a = xp[0];
-                b = xp[4];
-                s = xs[m * xs_sm + kb] * w_scale;
-            }
-            const f32x4 part = block_sum(wv, widen(a, b));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(part[i], s, acc[t][i]);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s_c[wave][4 * g + i][16 * t + r] = acc[t][i];
-    __syncthreads();
+__device__ __forceinline__ void join_waves(const float (&s_c)[NWAVE][16][16 * MT + 1], const Epilogue &ep, int nt, int m0, int M, int N) {
+    const int tid = threadIdx.x;
     auto total = [&](int row, int mm) {
         float y = 0.f;
 #pragma unroll
@@ -232,6 +220,185 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_kernel(const uint8_t *_
     }
 }
 
+// ---- any size: one tile of 16 weight rows and 16 MT rows of x per workgroup
+//
+// The waves cut K into slices and walk them in groups of PF blocks, weights and rows of x requested together, a group ahead; their
+// sums are joined through LDS.  x is read once per tile of weights, from L2: for rows too long to stay in registers.
+template <int NWAVE, int PF, int MT, bool EXACT, bool GLU>
+__global__ __launch_bounds__(NWAVE * 64) void linear_fp8_stream_kernel(const uint8_t *__restrict__ x, int64_t x_sm, const float *__restrict__ xs,
+                                                                       int64_t xs_sm, const uint8_t *__restrict__ tiles,
+                                                                       const float *__restrict__ ws, Epilogue ep, int M, int N, int kb_count,
+                                                                       int n_tiles, int groups_m) {
+    __shared__ float s_c[NWAVE][16][16 * MT + 1];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, g = lane >> 4;
+    // workgroups go to the XCDs in turn: the groups of rows that take the same tile share an XCD and its L2
+    const int turn = (int)(blockIdx.x >> 3), m0 = turn % groups_m * 16 * MT, nt = turn / groups_m * 8 + (int)(blockIdx.x & 7);
+    if (nt >= n_tiles) return;
+    const int per = ((kb_count + NWAVE - 1) / NWAVE + PF - 1) / PF * PF, begin = wave * per, end = min(begin + per, kb_count);
+    const uint4 *tp = reinterpret_cast<const uint4 *>(tiles + (int64_t)nt * kb_count * kTileBytes) + lane;
+    const float *wsp = ws + (int64_t)nt * kb_count * 2 + (g >> 1);
+    // rows beyond M are read as the last one; what they give is not stored
+    const uint8_t *xp[MT];
+    const float *xsp[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int64_t m = min(m0 + 16 * t + r, M - 1);
+        xp[t] = x + m * x_sm + g * 16;
+        xsp[t] = xs + m * xs_sm;
+    }
+    struct Group {
+        uint4 wa[PF], wb[PF], xa[PF][MT], xb[PF][MT];
+        float ws[PF], xs[PF][MT];
+    };
+    // blocks beyond the slice are read as its last one and count nothing
+    auto fetch = [&](Group &f, int kb0) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            const int kb = min(kb0 + i, end - 1);
+            f.wa[i] = ha_load16_stream(tp + (int64_t)kb * (kTileBytes / 16));
+            f.wb[i] = ha_load16_stream(tp + (int64_t)kb * (kTileBytes / 16) + 64);
+            f.ws[i] = wsp[2 * kb];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                f.xa[i][t] = *reinterpret_cast<const uint4 *>(xp[t] + kb * HA_FP8_BLOCK);
+                f.xb[i][t] = *reinterpret_cast<const uint4 *>(xp[t] + kb * HA_FP8_BLOCK + 64);
+                f.xs[i][t] = xsp[t][kb];
+            }
+        }
+    };
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (begin < end) {
+        Group now, next;
+        fetch(now, begin);
+        for (int kb = begin; kb < end; kb += PF) {
+            if (kb + PF < end) fetch(next, kb + PF);
+#pragma unroll
+            for (int i = 0; i < PF; ++i) {
+                if (kb + i < end) {
+                    Operand<EXACT> w, v;
+                    w.take(now.wa[i], now.wb[i]);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        v.take(now.xa[i][t], now.xb[i][t]);
+                        const f32x4 part = Operand<EXACT>::product(w, v);
+                        const float s = now.xs[i][t] * now.ws[i];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(part[e], s, acc[t][e]);
+                    }
+                }
+            }
+            now = next;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s_c[wave][4 * g + i][16 * t + r] = acc[t][i];
+    __syncthreads();
+    join_waves<NWAVE, MT, GLU>(s_c, ep, nt, m0, M, N);
+}
+
+// ---- few rows: x in registers, the weights streamed once
+//
+// The waves of a workgroup cut K into slices of KW blocks; each keeps its slice of 16 MT rows of x in registers (as e4m3, 8
+// registers per block and 16 rows; widened when used) and walks the weight tiles blockIdx, blockIdx + step, ...: per tile KW
+// blocks of 2 KiB, consecutive in memory, requested a whole tile ahead.  The waves' sums are joined through LDS.  What bounds it is
+// the stream of weights; the conversions (16 per block and 16 rows) and the matrix instructions run under it.
+template <int NWAVE, int KW, int PF, int MT, bool WIDE, bool EXACT, bool GLU>
+__global__ __launch_bounds__(NWAVE * 64) void linear_fp8_rows_kernel(const uint8_t *__restrict__ x, int64_t x_sm, const float *__restrict__ xs,
+                                                                     int64_t xs_sm, const uint8_t *__restrict__ tiles,
+                                                                     const float *__restrict__ ws, Epilogue ep, int M, int N, int kb_count,
+                                                                     int n_tiles, int groups_m) {
+    static_assert(KW % PF == 0, "a slice is whole groups of blocks");
+    __shared__ float s_c[NWAVE][16][16 * MT + 1];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    // workgroups go to the XCDs in turn: the groups of rows that walk the same tiles share an XCD and its L2
+    const int turn = (int)(blockIdx.x >> 3), step = (int)(gridDim.x / (unsigned)groups_m);
+    const int m0 = turn % groups_m * 16 * MT, kb0 = wave * KW;
+    int nt = turn / groups_m * 8 + (int)(blockIdx.x & 7);
+
+    struct Group {
+        uint4 a[PF], b[PF];
+        float s[PF];
+    };
+    auto fetch = [&](Group &w, int nt, int j0) {
+        const int64_t tile = (int64_t)nt * kb_count + kb0 + j0;
+        const uint4 *tp = reinterpret_cast<const uint4 *>(tiles + tile * kTileBytes) + lane;
+        const float *sp = ws + tile * 2 + (g >> 1);
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            w.a[i] = w.b[i] = make_uint4(0u, 0u, 0u, 0u);
+            w.s[i] = 0.f;
+            if (nt < n_tiles && kb0 + j0 + i < kb_count) {
+                w.a[i] = ha_load16_stream(tp + i * (kTileBytes / 16));
+                w.b[i] = ha_load16_stream(tp + i * (kTileBytes / 16) + 64);
+                w.s[i] = sp[2 * i];
+            }
+        }
+    };
+    Group now, next;
+    fetch(now, nt, 0);  // the first weights are on their way before x is set up
+    uint4 xa[KW][MT], xb[KW][MT];
+    float xsc[KW][MT];
+#pragma unroll
+    for (int j = 0; j < KW; ++j)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int m = m0 + 16 * t + r;
+            xa[j][t] = xb[j][t] = make_uint4(0u, 0u, 0u, 0u);
+            xsc[j][t] = 0.f;
+            if (m < M && kb0 + j < kb_count) {
+                const uint4 *xp = reinterpret_cast<const uint4 *>(x + m * x_sm + (kb0 + j) * HA_FP8_BLOCK + g * 16);
+                xa[j][t] = xp[0];
+                xb[j][t] = xp[4];
+                xsc[j][t] = xs[m * xs_sm + kb0 + j];
+            }
+        }
+    while (nt < n_tiles) {
+        const int nt_next = nt + step;
+        if constexpr (EXACT && !WIDE) {  // the compiler would widen x once, in front of the loop, at twice the registers
+#pragma unroll
+            for (int j = 0; j < KW; ++j)
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                    asm volatile("" : "+v"(xa[j][t].x), "+v"(xa[j][t].y), "+v"(xa[j][t].z), "+v"(xa[j][t].w), "+v"(xb[j][t].x),
+                                 "+v"(xb[j][t].y), "+v"(xb[j][t].z), "+v"(xb[j][t].w));
+        }
+        f32x4 acc[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j0 = 0; j0 < KW; j0 += PF) {
+            if (j0 + PF < KW) fetch(next, nt, j0 + PF);
+            else fetch(next, nt_next, 0);  // nothing is requested past the last tile
+#pragma unroll
+            for (int i = 0; i < PF; ++i) {
+                Operand<EXACT> w, v;
+                w.take(now.a[i], now.b[i]);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    v.take(xa[j0 + i][t], xb[j0 + i][t]);
+                    const f32x4 part = Operand<EXACT>::product(w, v);
+                    const float s = xsc[j0 + i][t] * now.s[i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(part[e], s, acc[t][e]);
+                }
+            }
+            now = next;
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_c[wave][4 * g + i][16 * t + r] = acc[t][i];
+        __syncthreads();
+        join_waves<NWAVE, MT, GLU>(s_c, ep, nt, m0, M, N);
+        nt = nt_next;
+        if (nt < n_tiles) __syncthreads();  // the sums are read: the next tile's may overwrite them
+    }
+}
+
 // ---- many rows: tiles of BN weight rows x BM rows of x per workgroup, staged through LDS
 //
 // WN x WM waves of TN x TM operand tiles each (16 weight rows, 16 rows of x).  Everything a block of 128 inputs needs travels
@@ -243,30 +410,6 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_kernel(const uint8_t *_
 // Two buffers, each in two parts: x with the first half of every wave's weight tiles, and the second half.  A part is requested
 // as soon as all waves have read the part of two blocks before out of its place, half a block's time after the other: between
 // its request and its use lie one and a half blocks' time, and three quarters of the buffers are always on their way.
-// EXACT: bf16 matrix instructions on widened operands; otherwise the 8-bit ones (see the top of this file).
-template <bool EXACT>
-struct TileOperand;
-template <>
-struct TileOperand<false> {
-    i32x8 v;
-    __device__ __forceinline__ void load(const uint8_t *first, const uint8_t *second) {
-        const uint4 a = *reinterpret_cast<const uint4 *>(first), b = *reinterpret_cast<const uint4 *>(second);
-        v = i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
-    }
-    // constant zero scale operands select the instruction without block exponents
-    __device__ static __forceinline__ f32x4 product(const TileOperand &w, const TileOperand &x) {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-    }
-};
-template <>
-struct TileOperand<true> {
-    Wide v;
-    __device__ __forceinline__ void load(const uint8_t *first, const uint8_t *second) {
-        v = widen(*reinterpret_cast<const uint4 *>(first), *reinterpret_cast<const uint4 *>(second));
-    }
-    __device__ static __forceinline__ f32x4 product(const TileOperand &w, const TileOperand &x) { return block_sum(w.v, x.v); }
-};
-
 // Requests from memory straight to LDS: lane l's 16 (4) bytes from base + offset + from, and i * kStep more for the i-th of a call,
 // land at lds + l * 16 (l * 4) + i * kStep; `from` and lds are uniform over the wave.  A buffer resource takes its base from four
 // scalar registers and `from` from a fifth, so that a request costs no address arithmetic; the instruction's own offset counts
@@ -369,21 +512,21 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     const uint32_t x_first = kWBytes + (wm * TM * 16 + r) * HA_FP8_BLOCK + ((g ^ r) & 7) * 16, x_second = x_first ^ 64;
     const uint32_t w_first = wn * TN * kTileBytes + lane * 16;
     constexpr int kAhead = AHEAD, kRing = kAhead + 1;  // tiles of weights read ahead of the one in use
-    TileOperand<EXACT> xo[TM], wo[kRing];
+    Operand<EXACT> xo[TM], wo[kRing];
     f32x4 part[2][TM];
     float s[TM], s_next[TM + 1];  // of the next block as they lie in LDS: rows of x, weights
     auto load_row = [&](int kb, int u) {
         const uint8_t *b = &s_buf[0][0] + (kb & 1) * kBuffer + u * kTileBytes;
-        xo[u].load(b + x_first, b + x_second);
+        xo[u].take(*reinterpret_cast<const uint4 *>(b + x_first), *reinterpret_cast<const uint4 *>(b + x_second));
     };
     auto load_scales = [&](int kb) {
         s_next[TM] = s_ws[kb & 1][wave * 64 + lane];
 #pragma unroll
         for (int u = 0; u < TM; ++u) s_next[u] = s_xs[kb & 1][(wm * TM + u) * 16 + r];
     };
-    auto load_weights = [&](TileOperand<EXACT> &w, int kb, int t) {
+    auto load_weights = [&](Operand<EXACT> &w, int kb, int t) {
         const uint8_t *b = &s_buf[0][0] + (kb & 1) * kBuffer + w_first + t * kTileBytes;
-        w.load(b, b + 1024);
+        w.take(*reinterpret_cast<const uint4 *>(b), *reinterpret_cast<const uint4 *>(b + 1024));
     };
     static_assert(TN % kRing == 0 && kAhead < TH, "a block ends on the operand register it began with; its halves are further apart");
     // the order of requests: of every block x, scales, first half, then the second half
@@ -428,7 +571,7 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
             if (t == TN - 1) load_scales(kb + 1);
 #pragma unroll
             for (int u = 0; u < TM; ++u) {
-                part[t & 1][u] = TileOperand<EXACT>::product(wo[t % kRing], xo[u]);
+                part[t & 1][u] = Operand<EXACT>::product(wo[t % kRing], xo[u]);
                 if (t == TN - 1) load_row(kb + 1, u);
                 if (t > 0) {
 #pragma unroll
@@ -500,6 +643,69 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     }
 }
 
+struct Args {
+    hipStream_t stream;
+    const uint8_t *x;
+    int64_t x_sm;
+    const float *xs;
+    int64_t xs_sm;
+    const uint8_t *tiles;
+    const float *ws;
+    Epilogue ep;
+    int M, N, act;
+    Packed p;
+};
+
+// One workgroup per CU (PER_CU of them), in as even a number of tiles as it goes, in whole runs of 8 (the XCDs) per group of rows
+template <int NWAVE, int KW, int PF, int MT, bool WIDE, bool EXACT, int PER_CU = 1>
+void launch_rows(const Args &a) {
+    const int groups = (a.M + 16 * MT - 1) / (16 * MT);
+    const int rounds = (int)(((int64_t)a.p.n_tiles * groups + 256 * PER_CU - 1) / (256 * PER_CU));
+    const unsigned grid = (unsigned)groups * (unsigned)(((a.p.n_tiles + rounds - 1) / rounds + 7) / 8 * 8);
+    if (a.act)
+        hipLaunchKernelGGL((linear_fp8_rows_kernel<NWAVE, KW, PF, MT, WIDE, EXACT, true>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x,
+                           a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, groups);
+    else
+        hipLaunchKernelGGL((linear_fp8_rows_kernel<NWAVE, KW, PF, MT, WIDE, EXACT, false>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x,
+                           a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, groups);
+}
+
+template <int NWAVE, int PF, int MT, bool EXACT>
+void launch_stream(const Args &a) {
+    const int groups = (a.M + 16 * MT - 1) / (16 * MT);
+    const unsigned grid = (unsigned)groups * (unsigned)((a.p.n_tiles + 7) / 8 * 8);
+    if (a.act)
+        hipLaunchKernelGGL((linear_fp8_stream_kernel<NWAVE, PF, MT, EXACT, true>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x, a.x_sm,
+                           a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, groups);
+    else
+        hipLaunchKernelGGL((linear_fp8_stream_kernel<NWAVE, PF, MT, EXACT, false>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x, a.x_sm,
+                           a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, groups);
+}
+
+template <int WN, int WM, int TN, int TM, int AHEAD, bool EXACT>
+void launch_tiled(const Args &a) {
+    const int tiles_n = (a.p.n_tiles + WN * TN - 1) / (WN * TN), tiles_m = (a.M + 16 * WM * TM - 1) / (16 * WM * TM);
+    const int per_xcd = (int)(((int64_t)tiles_n * tiles_m + 7) / 8);
+    if (a.act)
+        hipLaunchKernelGGL((linear_fp8_tiled_kernel<WN, WM, TN, TM, AHEAD, EXACT, true>), dim3(8u * (unsigned)per_xcd), dim3(WN * WM * 64), 0,
+                           a.stream, a.x, a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, tiles_n, tiles_m, per_xcd);
+    else
+        hipLaunchKernelGGL((linear_fp8_tiled_kernel<WN, WM, TN, TM, AHEAD, EXACT, false>), dim3(8u * (unsigned)per_xcd), dim3(WN * WM * 64), 0,
+                           a.stream, a.x, a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, tiles_n, tiles_m, per_xcd);
+}
+
+// 17 to 128 rows (and more where tiles do not apply)
+template <bool EXACT>
+void launch_some_rows(const Args &a) {
+    if (a.p.kb <= 32) {
+        if (a.M <= 32) launch_rows<8, 4, 4, 2, false, EXACT>(a);
+        else launch_rows<8, 4, 2, 4, false, EXACT>(a);
+    } else {
+        if (a.M <= 32) launch_stream<8, 2, 2, EXACT>(a);
+        else launch_stream<8, 2, 4, EXACT>(a);
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -558,45 +764,29 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
     if (st || M == 0) return st;
     const bool wide = ha_aligned(out, 4 * es) && out_stride_m % 4 == 0 && (!residual || (ha_aligned(residual, 4 * es) && residual_stride_m % 4 == 0));
     const Epilogue ep = {residual, residual_stride_m, out, out_stride_m, out_dtype, wide, ha_aligned(out, 8 * es) && out_stride_m % 8 == 0};
-    if (M > 128 && 256 * (xq_stride_m + x_scales_stride_m * 4) < (1LL << 31) && (int64_t)p.kb * kTileBytes * 16 < (1LL << 31)) {
-        const bool exact = out_dtype == HA_F32;
+    const Args a = {(hipStream_t)stream, (const uint8_t *)xq, xq_stride_m, x_scales, x_scales_stride_m, (const uint8_t *)tiles, tile_scales, ep,
+                    M, N, act, p};
+    const bool exact = out_dtype == HA_F32;
+    HA_REQUIRE(((int64_t)M + 15) / 16 * (p.n_tiles + 7LL) <= 2147483647LL, HA_ERR_BAD_SHAPE, "too many tiles for one launch");
+    // offsets within a workgroup's tiles are 32-bit
+    const bool tiled = M > 128 && 256 * (xq_stride_m + x_scales_stride_m * 4) < (1LL << 31) && (int64_t)p.kb * kTileBytes * 16 < (1LL << 31);
+    if (tiled) {
         const int64_t big = ((p.n_tiles + 15LL) / 16) * ((M + 255LL) / 256);
-        const bool use_big = !exact && big >= 200;
-        const int tiles_n = use_big ? (p.n_tiles + 15) / 16 : (p.n_tiles + 7) / 8, tiles_m = use_big ? (M + 255) / 256 : (M + 127) / 128;
-        const int64_t total = (int64_t)tiles_n * tiles_m, per_xcd = (total + 7) / 8;
-        HA_REQUIRE(total <= 2147483647LL / 8, HA_ERR_BAD_SHAPE, "too many tiles for one launch");
-#define HA_TILED(WN_, WM_, TN_, TM_, A_, E_, G_)                                                                                             \
-    hipLaunchKernelGGL((linear_fp8_tiled_kernel<WN_, WM_, TN_, TM_, A_, E_, G_>), dim3((unsigned)(8 * per_xcd)), dim3(WN_ * WM_ * 64), 0,    \
-                       (hipStream_t)stream, (const uint8_t *)xq, xq_stride_m, x_scales, x_scales_stride_m, (const uint8_t *)tiles,       \
-                       tile_scales, ep, M, N, p.kb, p.n_tiles, tiles_n, tiles_m, (int)per_xcd)
-        if (exact && act) HA_TILED(2, 2, 4, 4, 1, true, true);
-        else if (exact) HA_TILED(2, 2, 4, 4, 1, true, false);
-        else if (use_big && act) HA_TILED(2, 4, 8, 4, 3, false, true);
-        else if (use_big) HA_TILED(2, 4, 8, 4, 3, false, false);
-        else if (act) HA_TILED(2, 2, 4, 4, 1, false, true);
-        else HA_TILED(2, 2, 4, 4, 1, false, false);
-#undef HA_TILED
-        HA_CHECK_LAUNCH("linear_fp8_tiled_kernel");
-        return HA_OK;
-    }
-    const int MT = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-    const int64_t grid = (int64_t)p.n_tiles * ((M + 16LL * MT - 1) / (16 * MT));
-    HA_REQUIRE(grid <= 2147483647LL, HA_ERR_BAD_SHAPE, "too many tiles for one launch");
-#define HA_LINEAR(NW_, MT_, G_)                                                                                                          \
-    hipLaunchKernelGGL((linear_fp8_kernel<NW_, MT_, G_>), dim3((unsigned)grid), dim3(NW_ * 64), 0, (hipStream_t)stream, (const uint8_t *)xq, \
-                       xq_stride_m, x_scales, x_scales_stride_m, (const uint8_t *)tiles, tile_scales, ep, M, N, p.kb, p.n_tiles)
-    if (MT == 1) {
-        if (act) HA_LINEAR(8, 1, true);
-        else HA_LINEAR(8, 1, false);
-    } else if (MT == 2) {
-        if (act) HA_LINEAR(8, 2, true);
-        else HA_LINEAR(8, 2, false);
+        if (exact) launch_tiled<2, 2, 4, 4, 1, true>(a);
+        else if (big >= 200) launch_tiled<2, 4, 8, 4, 3, false>(a);
+        else launch_tiled<2, 2, 4, 4, 1, false>(a);
+    } else if (M <= 16) {
+        if (p.kb <= 8) launch_rows<8, 1, 1, 1, true, true>(a);
+        else if (p.kb <= 16) launch_rows<8, 2, 2, 1, true, true>(a);
+        else if (p.kb <= 32 && p.n_tiles < 1024) launch_rows<8, 4, 4, 1, true, true>(a);
+        else if (p.kb <= 32) launch_rows<8, 4, 2, 1, false, true, 2>(a);
+        else launch_stream<16, 2, 1, true>(a);
+    } else if (exact) {
+        launch_some_rows<true>(a);
     } else {
-        if (act) HA_LINEAR(8, 4, true);
-        else HA_LINEAR(8, 4, false);
+        launch_some_rows<false>(a);
     }
-#undef HA_LINEAR
-    HA_CHECK_LAUNCH("linear_fp8_kernel");
+    HA_CHECK_LAUNCH("ha_linear_fp8");
     return HA_OK;
 }
 

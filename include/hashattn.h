@@ -528,8 +528,10 @@ int ha_linear_tiled(const void *x, int64_t x_stride_m, const void *tiles, const 
  *
  * ha_linear_fp8: out [M, N] = x . W^T (+ residual [M, N] of out_dtype), or with act = HA_ACT_SWIGLU (weights packed with glu = 1)
  * out [M, N / 2] = silu(gate) * up.  Products exact, sums in fp32, ONE rounding to out_dtype at the end (residual and SwiGLU before
- * it).  Any M, N, K; `residual` may be `out` itself.  Which kernel runs depends on the sizes alone; a row's outputs do not
- * depend on the other rows.
+ * it).  16-bit results of more than 16 rows are summed by the 8-bit matrix instructions, which drop what lies more than 13 bits
+ * below the largest of eight neighbouring products: about 1.5e-5 of the result, where the result's own rounding is 2^-9 or 2^-12 of
+ * it.  Any M, N, K; `residual` may be `out` itself.  Which kernel runs depends on the sizes, out_dtype and strides alone; a row's
+ * outputs do not depend on the other rows' values.
  */
 #define HA_FP8_BLOCK 128
 #define HA_FP8_E4M3 3 /* dtype code of ha_pack_weight_fp8 only */

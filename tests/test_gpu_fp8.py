@@ -200,8 +200,8 @@ def make_linear(m, n, k, seed=0, glu=False, outlier=True):
 
 
 def eight_bit_sums(m, out_dtype):
-    """16-bit results of more than 128 rows run on the 8-bit matrix instructions."""
-    return m > 128 and out_dtype != torch.float32
+    """16-bit results of more than 16 rows run on the 8-bit matrix instructions."""
+    return m > 16 and out_dtype != torch.float32
 
 
 LINEAR_SIZES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (4, 6144, 4096), (4, 4096, 14336), (15, 100, 300), (16, 256, 1111), (17, 130, 257),
