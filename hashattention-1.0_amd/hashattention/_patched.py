@@ -31,6 +31,7 @@ from torch import nn
 from . import _ops
 from .cache import PreallocatedLayer, adopt_dynamic_layer
 from .decode import HashDecodeLayer
+from .fp8 import Fp8Linear, _stacks, stacked_weight
 
 DECODE_MAX_Q_LEN = 128   # reference: `if q_len > 128 or self.train_usa` routes to the original forward (:529)
 DEFAULT_USA_CFG = {"lth_int_dim": 128, "lth_final_dim": 32, "lth_thold": 0}     # reference :68-72
@@ -301,6 +302,13 @@ class USA(nn.Module):
         span = (D - 2 * ham.to(torch.int32)).to(K.dtype)
         span = torch.where(causal, span, torch.full([], torch.finfo(span.dtype).min, dtype=span.dtype, device=K.device))
         return span, ksign.to(K.dtype)
+
+
+def _fp8_projections(attn: nn.Module) -> bool:
+    """Whether an attention module's four projections are in 8 bits (`fp8.convert_fp8`) and q, k and v stack into one matrix."""
+    own = attn._modules
+    return all(type(own.get(n)) is Fp8Linear for n in ("q_proj", "k_proj", "v_proj", "o_proj")) \
+        and _stacks([own["q_proj"], own["k_proj"], own["v_proj"]])
 
 
 class HeavyHitterMixin:
@@ -591,12 +599,14 @@ class HeavyHitterMixin:
         if q_len != 1 or hidden % 32 or self.head_dim != 128 or hidden_states.dtype != torch.bfloat16 \
                 or not hidden_states.is_contiguous() or position_embeddings is None:
             return None
-        own = self._modules     # plain nn.Linear projections only: a wrapper around one (an adapter) has a forward of its own
-        if any(type(own.get(n)) is not nn.Linear for n in ("q_proj", "k_proj", "v_proj", "o_proj")):
+        own = self._modules     # plain nn.Linear (or 8-bit) projections only: a wrapper around one (an adapter) has a forward of its own
+        fp8 = _fp8_projections(self)
+        if not fp8 and any(type(own.get(n)) is not nn.Linear for n in ("q_proj", "k_proj", "v_proj", "o_proj")):
             return None
-        if any(own[n].bias is not None for n in ("q_proj", "k_proj", "v_proj", "o_proj")) or self.q_proj.weight.dtype != torch.bfloat16:
+        if any(own[n].bias is not None for n in ("q_proj", "k_proj", "v_proj", "o_proj")) or not fp8 and self.q_proj.weight.dtype != torch.bfloat16:
             return None
-        if self.q_proj.weight.device != hidden_states.device:       # a model spread over devices: its own hooks move the inputs
+        # a model spread over devices: its own hooks move the inputs
+        if (self.q_proj.tiles if fp8 else self.q_proj.weight).device != hidden_states.device:
             return None
         usa = self.usa_module
         if usa is None or usa.rehash_every_step or getattr(cache, "offloading", False):
@@ -630,7 +640,8 @@ class HeavyHitterMixin:
         (ha_linear_skinny; the library's GEMM on the stacked weight for more than 16 sequences), rotary embedding + in-place cache append + both hashes (ha_rope_encode_step_cos_sin), distance
         histograms, selection fused into the gather attention, output projection.  For the decoder layer around it
         (`fast_decoder_layer_forward`): `norm` = (weight, eps) of an RMSNorm applied to hidden_states inside the QKV projection,
-        `residual` [b, hidden] added inside the output projection."""
+        `residual` [b, hidden] added inside the output projection.  Projections in 8 bits (`fp8.convert_fp8`): the norm (or the
+        hidden states as they are) and the attention output go to 8 bits in a launch of their own in front of each."""
         b, _, hidden = hidden_states.shape
         H, Hkv, d = self.num_heads, self.num_key_value_heads, self.head_dim
         dev = hidden_states.device
@@ -640,8 +651,17 @@ class HeavyHitterMixin:
                       q=torch.empty(b, H, d, dtype=torch.bfloat16, device=dev),
                       attn=torch.empty(b, H, d, dtype=torch.bfloat16, device=dev))
             self.__dict__["_fast_scratch"] = sc
-        tiled = self._takes_tiled_projections(b, hidden)
-        if tiled:                               # 9 to 32 sequences: the matrix cores on a tiled copy of the stacked weight
+        fp8 = _fp8_projections(self)
+        tiled = not fp8 and self._takes_tiled_projections(b, hidden)
+        if fp8:
+            if "q8" not in sc:
+                sc["q8"], sc["a8"] = _ops.fp8_rows(b, hidden, dev), _ops.fp8_rows(b, H * d, dev)
+            if norm is None:
+                _ops.quantize_rows_fp8(hidden_states[:, 0, :], *sc["q8"])
+            else:
+                _ops.rmsnorm_fp8(hidden_states[:, 0, :], norm[0], norm[1], *sc["q8"])
+            _ops.linear_fp8(*sc["q8"], stacked_weight(self, "_qkv_fp8", (self.q_proj, self.k_proj, self.v_proj)), sc["qkv"])
+        elif tiled:                             # 9 to 32 sequences: the matrix cores on a tiled copy of the stacked weight
             _ops._linear_tiled_unchecked(hidden_states[:, 0, :], self._weight_tiles("_qkv_tiles", (self.q_proj.weight, self.k_proj.weight,
                                                                                                  self.v_proj.weight)),
                                          sc["qkv"].shape[1], sc["qkv"])
@@ -672,7 +692,10 @@ class HeavyHitterMixin:
         finally:
             hl.heavy_budget = saved
         out = torch.empty(b, 1, hidden, dtype=torch.bfloat16, device=dev)
-        if tiled:
+        if fp8:
+            _ops.quantize_rows_fp8(sc["attn"].view(b, H * d), *sc["a8"])
+            _ops.linear_fp8(*sc["a8"], self.o_proj.packed, out.view(b, hidden), residual=residual)
+        elif tiled:
             _ops._linear_tiled_unchecked(sc["attn"].view(b, H * d), self._weight_tiles("_o_tiles", (self.o_proj.weight,)), hidden,
                                          out.view(b, hidden), residual=residual)
         elif b > _ops.LINEAR_SKINNY_MAX_ROWS:
@@ -909,7 +932,7 @@ def _stacked_gate_up(attn, mlp) -> torch.Tensor:
 
 def _layer_modules(layer):
     """(mlp, input norm, post-attention norm, gate, up, down) of a decoder layer of the Llama shape - RMSNorm, attention,
-    residual, RMSNorm, SiLU-gated MLP of plain nn.Linear projections without biases, residual - or False.  Looked up once
+    residual, RMSNorm, SiLU-gated MLP of plain nn.Linear (or all `Fp8Linear`) projections without biases, residual - or False.  Looked up once
     and again whenever one of these modules is no longer the object that was looked at (an adapter library replaces
     projections by wrappers with a forward of their own; such a layer keeps the library's path)."""
     seen = layer.__dict__.get("_fast_seen")
@@ -921,7 +944,9 @@ def _layer_modules(layer):
         return seen[1]
     n1, n2, lin = now[1], now[2], now[3:]
     act = getattr(mlp, "act_fn", None)      # nn.SiLU, or the class transformers keeps under "silu"
-    ok = mlp is not None and n1 is not None and n2 is not None and all(type(m) is nn.Linear and m.bias is None for m in lin) \
+    kind = Fp8Linear if type(lin[0]) is Fp8Linear else nn.Linear
+    ok = mlp is not None and n1 is not None and n2 is not None and all(type(m) is kind and m.bias is None for m in lin) \
+        and (kind is nn.Linear or _stacks(lin[:2])) \
         and (isinstance(act, nn.SiLU) or type(act).__name__ == "SiLUActivation") \
         and all(getattr(n, "weight", None) is not None and hasattr(n, "variance_epsilon") and "RMSNorm" in type(n).__name__ for n in (n1, n2))
     layer.__dict__["_fast_seen"] = (now, now if ok else False)
@@ -947,6 +972,10 @@ def _layer_takes_fast_path(layer, hidden_states):
         if m._forward_hooks or m._forward_pre_hooks:
             return False
     gate, down = mods[3], mods[5]
+    if type(gate) is Fp8Linear:      # the 8-bit form takes any batch; attention and feed-forward half are of one kind
+        return mods if _fp8_projections(layer.self_attn) and mods[1].weight.dtype == mods[2].weight.dtype == torch.bfloat16 else False
+    if _fp8_projections(layer.self_attn):
+        return False
     if gate.in_features > 16384 and hidden_states.shape[0] <= FUSED_LAYER_MAX_ROWS:    # the norm-in-front form keeps a row of hidden states in registers
         return False
     bf16 = torch.bfloat16
@@ -975,6 +1004,26 @@ def fast_decoder_layer_forward(layer, hidden_states, attention_mask=None, positi
             attn._adopt_cache_layer(cache)
         attn._sync_bit_cache(cache)
         slot = attn._fast_decode_slot(hidden_states, position_embeddings, attention_mask, cache)
+        if slot is not None and type(mods[3]) is Fp8Linear:
+            # projections in 8 bits, any batch: twelve launches - norm to 8 bits, QKV, the attention step's three, its output to 8
+            # bits, output projection, the first residual's addition with the norm to 8 bits, gate/up, SwiGLU to 8 bits, and the down
+            # projection with the second residual inside
+            b, _, hidden = hidden_states.shape
+            mlp, n1, n2, gate, up, down = mods
+            a, _ = attn._fast_decode(hidden_states, position_embeddings, slot[0], norm=(n1.weight, float(n1.variance_epsilon)), amask=slot[1])
+            attn._note_key_storage(cache)
+            sc = attn.__dict__.get("_fast_fp8")
+            if sc is None or sc["gate_up"].shape != (b, 2 * gate.out_features) or sc["gate_up"].device != hidden_states.device:
+                sc = dict(gate_up=torch.empty(b, 2 * gate.out_features, dtype=torch.bfloat16, device=hidden_states.device),
+                          rows=_ops.fp8_rows(b, hidden, hidden_states.device), act=_ops.fp8_rows(b, gate.out_features, hidden_states.device))
+                attn.__dict__["_fast_fp8"] = sc
+            x1 = a[:, 0, :]     # the attention block's output becomes the residual stream in its own place
+            _ops.rmsnorm_fp8(x1, n2.weight, float(n2.variance_epsilon), *sc["rows"], residual=hidden_states[:, 0, :], sum_out=x1)
+            _ops.linear_fp8(*sc["rows"], stacked_weight(mlp, "_gate_up_fp8", (gate, up)), sc["gate_up"])
+            _ops.swiglu_fp8(sc["gate_up"], *sc["act"])
+            out = torch.empty_like(a)
+            _ops.linear_fp8(*sc["act"], down.packed, out[:, 0, :], residual=x1)
+            return out
         if slot is not None and hidden_states.shape[0] > FUSED_LAYER_MAX_ROWS:
             # more sequences than the fused forms take: the same layer in nine to twelve calls - each RMSNorm one launch with the
             # module's two roundings, the attention step (the first residual inside its output projection), gate/up with SwiGLU

@@ -29,13 +29,16 @@ class LlamaShapedDecoder:
     def __init__(self, n_layers=32, hidden=4096, ffn=14336, n_heads=32, n_kv_heads=8, head_dim=128, vocab=128256,
                  rope_theta=500000.0, rms_eps=1e-5, n_code_heads=8, lth_num_layers=3, lth_int_dim=128, lth_final_dim=32,
                  init_budget=128, recent_budget=128, heavy_budget=1.0 / 32, dtype=torch.bfloat16, device="cuda:0", seed=0,
-                 random_init=True):
+                 random_init=True, fp8_projections=False):
+        """fp8_projections: the four projections of every layer in 8 bits (`_ops.pack_weight_fp8`: e4m3, a scale per 128 x 128 block),
+        made at `allocate` from the weights the layer then holds, which are freed; lm_head, norms and caches keep `dtype`."""
         self.L, self.hidden, self.ffn, self.H, self.Hkv, self.d, self.vocab = n_layers, hidden, ffn, n_heads, n_kv_heads, head_dim, vocab
         self.theta, self.eps, self.dtype, self.device = rope_theta, rms_eps, dtype, torch.device(device)
         self.Hc = n_code_heads
         self.use_skinny = True   # ha_linear_skinny for the projections (bf16, batch <= 8) ...
         self.skinny_all = True   # ... including the down projection and the lm_head (False: library GEMMs for these two)
         self.tile_few_rows = True     # batches of up to 8: output and down projection from tiled copies of their weights
+        self.fp8 = bool(fp8_projections)
         self.fuse_rope = True    # ha_rope_encode_step instead of ha_rope_append + ha_encode_step
         self.usa_shape = (lth_num_layers, lth_int_dim, lth_final_dim)
         self.budgets = (init_budget, recent_budget, heavy_budget)
@@ -105,6 +108,10 @@ class LlamaShapedDecoder:
         self.pos_dev = torch.zeros(B, dtype=torch.int32, device=self.device)
         self.len_dev = torch.ones(B, dtype=torch.int32, device=self.device)
         self._gen_graph = self._gen_logits = None
+        if self.fp8:
+            self.rows8 = _ops.fp8_rows(B, self.hidden, self.device)
+            self.attn8 = _ops.fp8_rows(B, self.H * self.d, self.device)
+            self.act8 = _ops.fp8_rows(B, self.ffn, self.device)
         self.ws_dense = _ops.workspace(_ops.dense_decode_workspace_bytes(B, self.H, S_cap), self.device)
         self._pack_tiles()
 
@@ -112,10 +119,17 @@ class LlamaShapedDecoder:
         """9 to 32 sequences of a bf16 model: the projections whose inputs fit (QKV, output, gate/up) run on the matrix cores
         from tiled copies of their weights (`ha_linear_tiled`)."""
         B = getattr(self, "B", 0)
-        return self.use_skinny and self.dtype == torch.bfloat16 and B > 8 and _ops.linear_tiled_applies(B, max(self.hidden, self.H * self.d))
+        return not self.fp8 and self.use_skinny and self.dtype == torch.bfloat16 and B > 8 and _ops.linear_tiled_applies(B, max(self.hidden, self.H * self.d))
 
     def _pack_tiles(self) -> None:
-        """(Re)make the tiled copies for the batch this decoder was allocated for; dropped when they do not apply."""
+        """(Re)make the tiled copies for the batch this decoder was allocated for; dropped when they do not apply.  With
+        `fp8_projections` the 8-bit weights instead, once, in place of the ones they are made from."""
+        if self.fp8:
+            for p in self.layers:
+                for name in ("wqkv", "wo", "w13", "w2"):
+                    if name in p and p[name].numel():
+                        p[name + "_8"] = _ops.pack_weight_fp8(p.pop(name), glu=name == "w13")
+            return
         few = self.use_skinny and self.dtype == torch.bfloat16 and 0 < getattr(self, "B", 0) <= 8 and self.tile_few_rows
         for p in self.layers:
             for name in ("wqkv_t", "wo_t", "w13_t", "w2_t"):
@@ -187,7 +201,9 @@ class LlamaShapedDecoder:
 
         Per layer (bf16, up to 8 sequences): QKV projection with its RMSNorm folded in, ha_rope_append, the attention
         step, output projection with the residual folded in, gate/up projection with its RMSNorm and SwiGLU folded in,
-        down projection with the residual folded in.  Other dtypes and batches: the same steps as library calls plus
+        down projection with the residual folded in.  With `fp8_projections` (any batch): RMSNorm to 8 bits, QKV, the attention
+        step, its output to 8 bits, output projection, the residual's addition with the RMSNorm to 8 bits, gate/up with SwiGLU
+        inside, the activations to 8 bits, down projection with the residual inside.  Other dtypes and batches: the same steps as library calls plus
         ha_rmsnorm and ha_swiglu."""
         B, H, Hkv, d = self.B, self.H, self.Hkv, self.d
         if self.lengths is not None and not device_pos:
@@ -197,7 +213,7 @@ class LlamaShapedDecoder:
         x = self.embed[tokens]                                            # [B, hidden]
         # the row-streaming kernel against the library GEMM at B = 4: QKV 11.3 us (19.3), output projection 9.5 (19.1),
         # gate/up 40.9 (59.8), down projection 24.7 (25.1), lm_head 174.8 (184.7)
-        skinny = self.use_skinny and self.dtype == torch.bfloat16 and B <= 8
+        skinny = self.use_skinny and self.dtype == torch.bfloat16 and B <= 8 and not self.fp8
         # 16-bit models outside the fused forms keep their roundings: the norm's two (ha_rmsnorm), the projection's own before a
         # residual is added (efficiency/model.py:314-319, :190-191); fp32 has none to keep
         lowp = self.dtype != torch.float32
@@ -210,7 +226,10 @@ class LlamaShapedDecoder:
             return out
         tiled = self._tiled() and "wqkv_t" in self.layers[0]
         for l, p in enumerate(self.layers):
-            if skinny:      # RMSNorm rides in the projection that consumes it
+            if self.fp8:
+                _ops.rmsnorm_fp8(x, p["attn_norm"], self.eps, *self.rows8)
+                qkv = _ops.linear_fp8(*self.rows8, p["wqkv_8"], self.qkv)
+            elif skinny:    # RMSNorm rides in the projection that consumes it
                 qkv = _ops.linear_skinny(x, p["wqkv"], self.qkv, norm_weight=p["attn_norm"], eps=self.eps)
             elif tiled:
                 qkv = _ops.linear_tiled(norm(x, p["attn_norm"]), p["wqkv_t"], self.qkv.shape[1], self.qkv)
@@ -233,6 +252,15 @@ class LlamaShapedDecoder:
                 _ops.rope_append(qkv, H, Hkv, pos, self.inv_freq, self.q_rot, self.k_cache[l], self.v_cache[l])
                 hl.n_cached = pos
                 hl.step(self.q_rot.unsqueeze(2), self.k_cache[l], self.v_cache[l], S, self.attn_out)
+            if self.fp8:
+                _ops.quantize_rows_fp8(self.attn_out.view(B, H * d), *self.attn8)
+                a = _ops.linear_fp8(*self.attn8, p["wo_8"], self.x_attn[0])
+                # the sum takes the projection's place: x itself may still be the other buffer or the embedding's rows
+                _ops.rmsnorm_fp8(a, p["ffn_norm"], self.eps, *self.rows8, residual=x, sum_out=a)
+                _ops.linear_fp8(*self.rows8, p["w13_8"], self.ffn_act, swiglu=True)
+                _ops.quantize_rows_fp8(self.ffn_act, *self.act8)
+                x = _ops.linear_fp8(*self.act8, p["w2_8"], self.x_attn[1], residual=a)
+                continue
             if skinny:
                 # x lives in one of two buffers from here on (the down projection below adds in place)
                 xo = self.x_attn[0 if self.skinny_all else (l + 1) % 2]
@@ -263,7 +291,7 @@ class LlamaShapedDecoder:
                 x = x.addmm_(self.ffn_act, p["w2"].t())      # in place: the out-of-place form first copies x into its result
         if advance and not device_pos:
             self.seq_len = S
-        if skinny and self.skinny_all:
+        if (skinny or self.fp8 and self.use_skinny and self.dtype == torch.bfloat16 and B <= 8) and self.skinny_all:
             return _ops.linear_skinny(x, self.lm_head, self.logits, norm_weight=self.final_norm, eps=self.eps)
         return F.linear(norm(x, self.final_norm), self.lm_head)
 
@@ -324,10 +352,12 @@ class LlamaShapedDecoder:
 
     # ------------------------------------------------------------------ weights from a transformers Llama
     @classmethod
-    def from_hf(cls, model, usa_modules, batch: int, cache_len: int, dtype=torch.bfloat16, device="cuda:0") -> "LlamaShapedDecoder":
+    def from_hf(cls, model, usa_modules, batch: int, cache_len: int, dtype=torch.bfloat16, device="cuda:0",
+                fp8_projections: bool = False) -> "LlamaShapedDecoder":
         """The decoder for a `transformers` LlamaForCausalLM and the hash modules `load_usa` returned for it (one `USA` per
         layer): same weights, budgets from the model's config (`init_budget`, `heavy_budget`, `recent_budget`, as
-        `convert_usa` reads them), caches for `batch` sequences of up to `cache_len` tokens.  Follow with
+        `convert_usa` reads them), caches for `batch` sequences of up to `cache_len` tokens; `fp8_projections`: the layers'
+        projections in 8 bits.  Follow with
         `prefill_from_hf` and `generate`."""
         cfg, usa0 = model.config, usa_modules[0]
         if usa0.rehash_every_step:
@@ -346,7 +376,7 @@ class LlamaShapedDecoder:
                   n_kv_heads=cfg.num_key_value_heads, head_dim=head_dim, vocab=cfg.vocab_size, rms_eps=cfg.rms_norm_eps,
                   n_code_heads=usa0.num_heads, lth_num_layers=usa0.num_layers, lth_int_dim=usa0.int_dim, lth_final_dim=usa0.lth_final_dim,
                   init_budget=cfg.init_budget, recent_budget=cfg.recent_budget, heavy_budget=cfg.heavy_budget, dtype=dtype,
-                  device=device, random_init=False)
+                  device=device, random_init=False, fp8_projections=fp8_projections)
         dec.load_hf_llama(model)
         lin = lambda seqs: [[(m.weight.detach().float().cpu(), m.bias.detach().float().cpu()) for m in seq if isinstance(m, torch.nn.Linear)]
                             for seq in seqs]

@@ -1,0 +1,118 @@
+"""Projections in 8 bits for `transformers` models: e4m3 weights with one scale per 128 x 128 block, activations quantised per row and
+128 inputs on their way into each projection (`ha_linear_fp8` and the row operators in front of it).
+
+    model = convert_usa(model, config, usa, False, False)      # optional, and first
+    model = convert_fp8(model)                                 # every decoder layer's seven projections
+    model.generate(...)
+
+`convert_fp8` replaces the projections of every decoder layer of the Llama shape (q, k, v, o, gate, up, down) by `Fp8Linear` and frees
+the 16-bit weights: half the memory, half the bytes a decode step streams, and prompts on the 8-bit matrix instructions.  Norms,
+embeddings and the lm_head stay as they are.  A converted layer's single-token steps run as a fixed set of launches around
+`HeavyHitterMixin._fast_decode` (see `_patched.fast_decoder_layer_forward`).  Inference only.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+from torch import nn
+
+from . import _ops
+
+__all__ = ["Fp8Linear", "convert_fp8", "stacked_weight"]
+
+
+class Fp8Linear(nn.Module):
+    """`nn.Linear` for inference with its weight in 8 bits.  `tiles` and `tile_scales` are buffers (`_ops.pack_weight_fp8`), so the
+    module moves and is saved like any other."""
+
+    def __init__(self, weight: _ops.Fp8Weight, bias: Optional[torch.Tensor] = None):
+        super().__init__()
+        if weight.glu:
+            raise ValueError("interleaved gate/up weights have no plain product")
+        self.in_features, self.out_features = weight.K, weight.N
+        self.register_buffer("tiles", weight.tiles)
+        self.register_buffer("tile_scales", weight.scales)
+        self.register_buffer("bias", None if bias is None else bias.detach())
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "Fp8Linear":
+        return cls(_ops.pack_weight_fp8(linear.weight.detach()), linear.bias)
+
+    @property
+    def packed(self) -> _ops.Fp8Weight:
+        return _ops.Fp8Weight(self.tiles, self.tile_scales, self.out_features, self.in_features, False)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("Fp8Linear is for inference: no gradient flows through the 8-bit product (use torch.no_grad())")
+        rows = x.reshape(-1, self.in_features)
+        if self.in_features > 1 and rows.stride(1) != 1:
+            rows = rows.contiguous()
+        q, scales = _ops.fp8_rows(rows.shape[0], self.in_features, x.device)
+        _ops.quantize_rows_fp8(rows, q, scales)
+        out = torch.empty(rows.shape[0], self.out_features, dtype=x.dtype, device=x.device)
+        _ops.linear_fp8(q, scales, self.packed, out)
+        if self.bias is not None:
+            out += self.bias
+        return out.view(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, e4m3 per 128 x 128 block"
+
+
+def _stacks(modules: Sequence[Fp8Linear]) -> bool:
+    """Whether the modules' rows can lie behind each other in one packed matrix: whole tiles of 16 rows in front of the last."""
+    return all(m.out_features % 16 == 0 for m in modules[:-1]) and len({m.in_features for m in modules}) == 1
+
+
+def stacked_weight(owner: nn.Module, name: str, modules: Sequence[Fp8Linear]) -> _ops.Fp8Weight:
+    """The modules' weights as one matrix, rows behind each other, kept on `owner` under `name`.  Packed tiles are ordered by row, so
+    the modules' own buffers become parts of the stacked ones: nothing is held twice.  Rebuilt when a module's buffer was
+    replaced (a move to another device, a loaded state dict)."""
+    key = tuple(t.data_ptr() for m in modules for t in (m.tiles, m.tile_scales))
+    hit = owner.__dict__.get(name)
+    if hit is not None and hit[0] == key:
+        return hit[1]
+    if not _stacks(modules):
+        raise ValueError("rows of packed weights stack in whole tiles of 16")
+    tiles, scales = torch.cat([m.tiles for m in modules]), torch.cat([m.tile_scales for m in modules])
+    at = s_at = 0
+    for m in modules:
+        n, ns = m.tiles.numel(), m.tile_scales.numel()
+        m.tiles, m.tile_scales = tiles[at:at + n], scales[s_at:s_at + ns]
+        at, s_at = at + n, s_at + ns
+    weight = _ops.Fp8Weight(tiles, scales, sum(m.out_features for m in modules), modules[0].in_features, False)
+    owner.__dict__[name] = (tuple(t.data_ptr() for m in modules for t in (m.tiles, m.tile_scales)), weight)
+    return weight
+
+
+_ATTENTION, _MLP = ("q_proj", "k_proj", "v_proj", "o_proj"), ("gate_proj", "up_proj", "down_proj")
+
+
+def _is_layer(module: nn.Module) -> bool:
+    attn, mlp = getattr(module, "self_attn", None), getattr(module, "mlp", None)
+    return attn is not None and mlp is not None and all(isinstance(getattr(attn, n, None), nn.Linear) for n in _ATTENTION) \
+        and all(isinstance(getattr(mlp, n, None), nn.Linear) for n in _MLP)
+
+
+def convert_fp8(model: nn.Module) -> nn.Module:
+    """Replace the seven projections of every decoder layer in place by `Fp8Linear`.  The model is on the GPU; `convert_usa`, where it
+    is used, comes first (it copies 16-bit weights)."""
+    layers = [m for m in model.modules() if _is_layer(m)]
+    if not layers:
+        raise ValueError("no decoder layer with q/k/v/o and gate/up/down projections of type nn.Linear in this model")
+    for layer in layers:
+        attn, mlp = layer.self_attn, layer.mlp
+        # a converted attention module prefills through the module it replaced, which holds weights of its own
+        twin = getattr(getattr(attn, "flash_forward", None), "__self__", None)
+        for name in _ATTENTION:
+            new = Fp8Linear.from_linear(getattr(attn, name))
+            setattr(attn, name, new)
+            if twin is not None and isinstance(getattr(twin, name, None), nn.Linear):
+                setattr(twin, name, new)
+        for name in _MLP:
+            setattr(mlp, name, Fp8Linear.from_linear(getattr(mlp, name)))
+        for copy in ("_qkv_fused", "_qkv_tiles", "_o_tiles", "_gate_up_fused", "_gate_up_tiles", "_down_tiles"):
+            attn.__dict__.pop(copy, None)        # stacked and tiled copies of the 16-bit weights, if steps ran before
+    return model
