@@ -776,20 +776,24 @@ class Fp8Weight(NamedTuple):
     glu: bool
 
 
-def _same_device(*tensors):
-    """GPU tensors of one device; the launch then runs with that device as the current one."""
-    _require_cuda(*tensors)
-    dev = tensors[0].device
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _same_device(*tensors) -> int:
+    """The index of the one GPU the tensors (or None) live on."""
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError("tensors on different devices: " + ", ".join(str(t.device) for t in tensors if t is not None))
+    if dev < 0:
+        raise ValueError("hashattention ops take GPU tensors only (there is no CPU path)")
     return dev
 
 
-def _launch_on(dev, fn, where, *args):
-    """fn(*args, stream) on dev's current stream, with dev as the current device (a kernel launch takes the current one)."""
-    stream = _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
+def _launch_on(dev: int, fn, where: str, args: tuple) -> None:
+    """fn(*args, stream) on the current stream of GPU `dev`, with that GPU as the current one (a kernel launch takes the current one)."""
+    stream = _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+    if _current_device() == dev:
         st = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
@@ -814,35 +818,32 @@ def fp8_values(q: torch.Tensor, scales: torch.Tensor, k: int) -> torch.Tensor:
     return (q.float() * scales.repeat_interleave(FP8_BLOCK, dim=1))[:, :k]
 
 
-def _float_rows(t: torch.Tensor, m: int, k: int, what: str, dtype=None) -> None:
-    if t.dim() != 2 or t.shape[0] != m or t.shape[1] != k or (t.stride(1) != 1 and k > 1):
+def _rows_of(t: torch.Tensor, what: str, m: int, k: int, dtype=None) -> int:
+    """The row stride of t, checked to be [m, k] with contiguous rows of `dtype` (any floating type the kernels take, if None)."""
+    s0, s1 = t.stride() if t.dim() == 2 else (0, 0)
+    if t.shape != (m, k) or (s1 != 1 and k > 1):
         raise ValueError(f"{what} must be [{m}, {k}] with contiguous rows, got {tuple(t.shape)} with strides {t.stride()}")
-    if t.dtype not in _DTYPE or (dtype is not None and t.dtype != dtype):
+    if t.dtype != dtype if dtype is not None else t.dtype not in _DTYPE:
         raise ValueError(f"{what} is {t.dtype}" + (f", expected {dtype}" if dtype is not None else ""))
+    return s0 if m > 1 else max(s0, k)          # one row (or none) may carry any number there
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Stride of the rows; one row (or none) may carry any number there."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
-
-
-def _fp8_out(q: torch.Tensor, scales: torch.Tensor, m: int, k: int) -> Tuple[int, int]:
-    kb = fp8_blocks(k)
-    if q.dtype != torch.float8_e4m3fn or q.dim() != 2 or q.shape != (m, kb * FP8_BLOCK) or q.stride(1) != 1:
-        raise ValueError(f"q must be float8_e4m3fn [{m}, {kb * FP8_BLOCK}] with contiguous rows, got {q.dtype} {tuple(q.shape)}")
-    if scales.dtype != torch.float32 or scales.dim() != 2 or scales.shape != (m, kb) or (scales.stride(1) != 1 and kb > 1):
-        raise ValueError(f"scales must be fp32 [{m}, {kb}] with contiguous rows, got {scales.dtype} {tuple(scales.shape)}")
-    return _row_stride(q), _row_stride(scales)
+def _fp8_rows_of(q: torch.Tensor, scales: torch.Tensor, m: int, k: int) -> Tuple[int, int]:
+    """The row strides of m rows of k elements in 8 bits."""
+    kb = (k + 127) // 128
+    if q.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise ValueError(f"rows in 8 bits are float8_e4m3fn with fp32 scales, got {q.dtype} and {scales.dtype}")
+    return _rows_of(q, "q", m, kb * 128, torch.float8_e4m3fn), _rows_of(scales, "scales", m, kb, torch.float32)
 
 
 def quantize_rows_fp8(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor) -> None:
     """x [M, K] (fp32, bf16 or fp16) -> rows in 8 bits (`fp8_rows`), one scale per block of 128."""
     dev = _same_device(x, q, scales)
     m, k = x.shape
-    _float_rows(x, m, k, "x")
-    q_sm, s_sm = _fp8_out(q, scales, m, k)
-    _launch_on(dev, (_lib or load_library()).ha_quantize_rows_fp8, "ha_quantize_rows_fp8", x.data_ptr(), _row_stride(x), _DTYPE[x.dtype], m, k,
-               q.data_ptr(), q_sm, scales.data_ptr(), s_sm)
+    x_sm = _rows_of(x, "x", m, k)
+    q_sm, s_sm = _fp8_rows_of(q, scales, m, k)
+    _launch_on(dev, (_lib or load_library()).ha_quantize_rows_fp8, "ha_quantize_rows_fp8",
+               (x.data_ptr(), x_sm, _DTYPE[x.dtype], m, k, q.data_ptr(), q_sm, scales.data_ptr(), s_sm))
 
 
 def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, q: torch.Tensor, scales: torch.Tensor,
@@ -851,29 +852,31 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, q: torch.Tens
     layer's next addition; it may be x or residual itself."""
     dev = _same_device(x, weight, q, scales, residual, sum_out)
     m, k = x.shape
-    _float_rows(x, m, k, "x")
-    if weight.dtype != x.dtype or weight.shape != (k,) or not weight.is_contiguous():
-        raise ValueError(f"weight must be {x.dtype} [{k}], got {weight.dtype} {tuple(weight.shape)}")
+    dtype = x.dtype
+    x_sm = _rows_of(x, "x", m, k)
+    if weight.dtype != dtype or weight.shape != (k,) or not weight.is_contiguous():
+        raise ValueError(f"weight must be {dtype} [{k}], got {weight.dtype} {tuple(weight.shape)}")
+    r = h = None
+    r_sm = h_sm = 0
     if residual is not None:
-        _float_rows(residual, m, k, "residual", x.dtype)
+        r, r_sm = residual.data_ptr(), _rows_of(residual, "residual", m, k, dtype)
     if sum_out is not None:
-        _float_rows(sum_out, m, k, "sum_out", x.dtype)
-    q_sm, s_sm = _fp8_out(q, scales, m, k)
-    _launch_on(dev, (_lib or load_library()).ha_rmsnorm_fp8, "ha_rmsnorm_fp8", x.data_ptr(), _row_stride(x), _ptr(residual),
-               0 if residual is None else _row_stride(residual), weight.data_ptr(), _DTYPE[x.dtype], m, k, float(eps), _ptr(sum_out),
-               0 if sum_out is None else _row_stride(sum_out), q.data_ptr(), q_sm, scales.data_ptr(), s_sm)
+        h, h_sm = sum_out.data_ptr(), _rows_of(sum_out, "sum_out", m, k, dtype)
+    q_sm, s_sm = _fp8_rows_of(q, scales, m, k)
+    _launch_on(dev, (_lib or load_library()).ha_rmsnorm_fp8, "ha_rmsnorm_fp8",
+               (x.data_ptr(), x_sm, r, r_sm, weight.data_ptr(), _DTYPE[dtype], m, k, eps, h, h_sm, q.data_ptr(), q_sm, scales.data_ptr(), s_sm))
 
 
 def swiglu_fp8(gate_up: torch.Tensor, q: torch.Tensor, scales: torch.Tensor) -> None:
     """gate_up [M, 2 F] (gate | up) -> silu(gate) * up as rows of F in 8 bits."""
     dev = _same_device(gate_up, q, scales)
     m, k2 = gate_up.shape
-    _float_rows(gate_up, m, k2, "gate_up")
+    x_sm = _rows_of(gate_up, "gate_up", m, k2)
     if k2 % 2:
         raise ValueError(f"gate_up must hold an even number of columns, got {k2}")
-    q_sm, s_sm = _fp8_out(q, scales, m, k2 // 2)
-    _launch_on(dev, (_lib or load_library()).ha_swiglu_fp8, "ha_swiglu_fp8", gate_up.data_ptr(), _row_stride(gate_up), _DTYPE[gate_up.dtype], m,
-               k2 // 2, q.data_ptr(), q_sm, scales.data_ptr(), s_sm)
+    q_sm, s_sm = _fp8_rows_of(q, scales, m, k2 // 2)
+    _launch_on(dev, (_lib or load_library()).ha_swiglu_fp8, "ha_swiglu_fp8",
+               (gate_up.data_ptr(), x_sm, _DTYPE[gate_up.dtype], m, k2 // 2, q.data_ptr(), q_sm, scales.data_ptr(), s_sm))
 
 
 def pack_weight_fp8(w: torch.Tensor, scales: Optional[torch.Tensor] = None, glu: bool = False) -> Fp8Weight:
@@ -898,10 +901,12 @@ def pack_weight_fp8(w: torch.Tensor, scales: Optional[torch.Tensor] = None, glu:
     else:
         raise ValueError(f"w is {w.dtype}: fp32, bf16, fp16 or float8_e4m3fn")
     lib = load_library()
-    out = Fp8Weight(torch.empty(lib.ha_weight_fp8_bytes(n, k, int(glu)), dtype=torch.uint8, device=dev),
-                    torch.empty(lib.ha_weight_fp8_scales(n, k, int(glu)), dtype=torch.float32, device=dev), n, k, bool(glu))
-    _launch_on(dev, lib.ha_pack_weight_fp8, "ha_pack_weight_fp8", w.data_ptr(), _row_stride(w), dtype, _ptr(scales),
-               0 if scales is None else _row_stride(scales), n, k, int(glu), out.tiles.data_ptr(), out.scales.data_ptr())
+    out = Fp8Weight(torch.empty(lib.ha_weight_fp8_bytes(n, k, int(glu)), dtype=torch.uint8, device=w.device),
+                    torch.empty(lib.ha_weight_fp8_scales(n, k, int(glu)), dtype=torch.float32, device=w.device), n, k, bool(glu))
+    s_sn = 0 if scales is None else max(scales.stride(0), scales.shape[1]) if scales.shape[0] == 1 else scales.stride(0)
+    _launch_on(dev, lib.ha_pack_weight_fp8, "ha_pack_weight_fp8",
+               (w.data_ptr(), w.stride(0) if n > 1 else max(w.stride(0), k), dtype, _ptr(scales), s_sn, n, k, int(glu), out.tiles.data_ptr(),
+                out.scales.data_ptr()))
     return out
 
 
@@ -909,17 +914,19 @@ def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: to
                swiglu: bool = False) -> torch.Tensor:
     """out [M, N] = rows in 8 bits (q, scales) . W^T (+ residual), or [M, N / 2] = silu(gate) * up with swiglu (weights packed with
     glu); out fp32, bf16 or fp16, rounded once.  residual may be out itself."""
-    dev = _same_device(q, scales, weight.tiles, weight.scales, out, residual)
-    m, n = q.shape[0], weight.N
-    q_sm, s_sm = _fp8_out(q, scales, m, weight.K)
-    if weight.glu != swiglu:
+    tiles, tile_scales, n, k, glu = weight
+    dev = _same_device(q, scales, tiles, tile_scales, out, residual)
+    m = q.shape[0]
+    q_sm, s_sm = _fp8_rows_of(q, scales, m, k)
+    if glu != swiglu:
         raise ValueError("swiglu takes weights packed with glu, and nothing else does")
-    _float_rows(out, m, n // 2 if swiglu else n, "out")
+    o_sm = _rows_of(out, "out", m, n // 2 if swiglu else n)
+    r, r_sm = None, 0
     if residual is not None:
         if swiglu:
             raise ValueError("SwiGLU takes no residual")
-        _float_rows(residual, m, n, "residual", out.dtype)
-    _launch_on(dev, (_lib or load_library()).ha_linear_fp8, "ha_linear_fp8", q.data_ptr(), q_sm, scales.data_ptr(), s_sm, weight.tiles.data_ptr(),
-               weight.scales.data_ptr(), _ptr(residual), 0 if residual is None else _row_stride(residual),
-               HA_ACT_SWIGLU if swiglu else HA_ACT_NONE, out.data_ptr(), _row_stride(out), _DTYPE[out.dtype], m, n, weight.K)
+        r, r_sm = residual.data_ptr(), _rows_of(residual, "residual", m, n, out.dtype)
+    _launch_on(dev, (_lib or load_library()).ha_linear_fp8, "ha_linear_fp8",
+               (q.data_ptr(), q_sm, scales.data_ptr(), s_sm, tiles.data_ptr(), tile_scales.data_ptr(), r, r_sm, 1 if swiglu else 0,
+                out.data_ptr(), o_sm, _DTYPE[out.dtype], m, n, k))
     return out
