@@ -18,6 +18,7 @@
 
 namespace {
 
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -111,7 +112,7 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi) {
 struct Wide {
     bf16x8 v[4];
 };
-__device__ __forceinline__ Wide widen(const uint4 &a, const uint4 &b) {
+__device__ __forceinline__ Wide widen(const u32x4 &a, const u32x4 &b) {
     return {{widen8(a.x, a.y), widen8(a.z, a.w), widen8(b.x, b.y), widen8(b.z, b.w)}};
 }
 __device__ __forceinline__ f32x4 block_sum(const Wide &w, const Wide &x) {
@@ -128,8 +129,8 @@ struct Operand;
 template <>
 struct Operand<false> {
     i32x8 v;
-    __device__ __forceinline__ void take(const uint4 &a, const uint4 &b) {
-        v = i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+    __device__ __forceinline__ void take(const u32x4 &a, const u32x4 &b) {
+        v = __builtin_bit_cast(i32x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     // constant zero scale operands select the instruction without block exponents
     __device__ static __forceinline__ f32x4 product(const Operand &w, const Operand &x) {
@@ -139,7 +140,7 @@ struct Operand<false> {
 template <>
 struct Operand<true> {
     Wide v;
-    __device__ __forceinline__ void take(const uint4 &a, const uint4 &b) { v = widen(a, b); }
+    __device__ __forceinline__ void take(const u32x4 &a, const u32x4 &b) { v = widen(a, b); }
     __device__ static __forceinline__ f32x4 product(const Operand &w, const Operand &x) { return block_sum(w.v, x.v); }
 };
 
@@ -192,9 +193,9 @@ __device__ __forceinline__ void store4(const Epilogue &ep, int64_t m, int n, int
         if (n + i < cols) o[i] = y[i];
 }
 
-// The waves' sums of tile nt (s_c[wave][weight row][row of x]) joined, finished and stored by the whole workgroup.
-template <int NWAVE, int MT, bool GLU>
-__device__ __forceinline__ void join_waves(const float (&s_c)[NWAVE][16][16 * MT + 1], const Epilogue &ep, int nt, int m0, int M, int N) {
+// The waves' sums of NT tiles from nt on (s_c[wave][weight row][row of x]) joined, finished and stored by the whole workgroup.
+template <int NWAVE, int NT, int MT, bool GLU>
+__device__ __forceinline__ void join_waves(const float (&s_c)[NWAVE][16 * NT][16 * MT + 1], const Epilogue &ep, int nt, int m0, int M, int N) {
     const int tid = threadIdx.x;
     auto total = [&](int row, int mm) {
         float y = 0.f;
@@ -203,15 +204,16 @@ __device__ __forceinline__ void join_waves(const float (&s_c)[NWAVE][16][16 * MT
         return y;
     };
     if constexpr (GLU) {
-        for (int t = tid; t < 8 * 16 * MT; t += NWAVE * 64) {
-            const int mm = t >> 3, c = t & 7, col = 8 * nt + c;
+        for (int t = tid; t < 8 * NT * 16 * MT; t += NWAVE * 64) {
+            const int mm = t / (8 * NT), c = t % (8 * NT), col = 8 * nt + c;
             if (m0 + mm >= M || col >= N / 2) continue;
-            const float gate = total(c, mm);
-            ha_store_elem(ep.out, (m0 + mm) * ep.out_sm + col, gate / (1.0f + expf(-gate)) * total(8 + c, mm), ep.out_dtype);
+            const int row = (c >> 3) * 16 + (c & 7);
+            const float gate = total(row, mm);
+            ha_store_elem(ep.out, (m0 + mm) * ep.out_sm + col, gate / (1.0f + expf(-gate)) * total(row + 8, mm), ep.out_dtype);
         }
     } else {
-        for (int t = tid; t < 16 * 16 * MT; t += NWAVE * 64) {
-            const int mm = t >> 4, c = t & 15, n = 16 * nt + c;
+        for (int t = tid; t < 16 * NT * 16 * MT; t += NWAVE * 64) {
+            const int mm = t / (16 * NT), c = t % (16 * NT), n = 16 * nt + c;
             if (m0 + mm >= M || n >= N) continue;
             float y = total(c, mm);
             if (ep.res) y += ha_load_elem(ep.res, (m0 + mm) * ep.res_sm + n, ep.out_dtype);
@@ -220,24 +222,31 @@ __device__ __forceinline__ void join_waves(const float (&s_c)[NWAVE][16][16 * MT
     }
 }
 
-// ---- any size: one tile of 16 weight rows and 16 MT rows of x per workgroup
+// ---- any size: NT tiles of 16 weight rows and 16 MT rows of x per workgroup, straight from memory to registers
 //
-// The waves cut K into slices and walk them in groups of PF blocks, weights and rows of x requested together, a group ahead; their
-// sums are joined through LDS.  x is read once per tile of weights, from L2: for rows too long to stay in registers.
-template <int NWAVE, int PF, int MT, bool EXACT, bool GLU>
+// The waves cut K into slices and walk them in groups of PF blocks, weights and rows of x requested together, a group ahead, without
+// a barrier; their sums are joined through LDS.  Eight waves with a block or two each on its way keep more bytes in flight than
+// staging through LDS would, which is what a matrix of few tiles needs; NT and MT set how often x and the weights are read from L2.
+template <int NWAVE, int PF, int NT, int MT, bool EXACT, bool GLU>
 __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_stream_kernel(const uint8_t *__restrict__ x, int64_t x_sm, const float *__restrict__ xs,
                                                                        int64_t xs_sm, const uint8_t *__restrict__ tiles,
                                                                        const float *__restrict__ ws, Epilogue ep, int M, int N, int kb_count,
                                                                        int n_tiles, int groups_m) {
-    __shared__ float s_c[NWAVE][16][16 * MT + 1];
+    __shared__ float s_c[NWAVE][16 * NT][16 * MT + 1];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, g = lane >> 4;
-    // workgroups go to the XCDs in turn: the groups of rows that take the same tile share an XCD and its L2
-    const int turn = (int)(blockIdx.x >> 3), m0 = turn % groups_m * 16 * MT, nt = turn / groups_m * 8 + (int)(blockIdx.x & 7);
+    // workgroups go to the XCDs in turn: the groups of rows that take the same tiles share an XCD and its L2
+    const int turn = (int)(blockIdx.x >> 3), m0 = turn % groups_m * 16 * MT, nt = (turn / groups_m * 8 + (int)(blockIdx.x & 7)) * NT;
     if (nt >= n_tiles) return;
     const int per = ((kb_count + NWAVE - 1) / NWAVE + PF - 1) / PF * PF, begin = wave * per, end = min(begin + per, kb_count);
-    const uint4 *tp = reinterpret_cast<const uint4 *>(tiles + (int64_t)nt * kb_count * kTileBytes) + lane;
-    const float *wsp = ws + (int64_t)nt * kb_count * 2 + (g >> 1);
-    // rows beyond M are read as the last one; what they give is not stored
+    // rows beyond M and tiles beyond the matrix are read as the last ones; what they give is not stored
+    const u32x4 *tp[NT];
+    const float *wsp[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t tile = (int64_t)min(nt + j, n_tiles - 1) * kb_count;
+        tp[j] = reinterpret_cast<const u32x4 *>(tiles + tile * kTileBytes);
+        wsp[j] = ws + tile * 2;
+    }
     const uint8_t *xp[MT];
     const float *xsp[MT];
 #pragma unroll
@@ -247,57 +256,74 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_stream_kernel(const uin
         xsp[t] = xs + m * xs_sm;
     }
     struct Group {
-        uint4 wa[PF], wb[PF], xa[PF][MT], xb[PF][MT];
-        float ws[PF], xs[PF][MT];
+        u32x4 wa[PF][NT], wb[PF][NT], xa[PF][MT], xb[PF][MT];
+        float ws[PF][NT], xs[PF][MT];
     };
     // blocks beyond the slice are read as its last one and count nothing
-    auto fetch = [&](Group &f, int kb0) {
+    auto fetch = [&](Group &f, int kb0) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
             const int kb = min(kb0 + i, end - 1);
-            f.wa[i] = ha_load16_stream(tp + (int64_t)kb * (kTileBytes / 16));
-            f.wb[i] = ha_load16_stream(tp + (int64_t)kb * (kTileBytes / 16) + 64);
-            f.ws[i] = wsp[2 * kb];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                f.wa[i][j] = __builtin_nontemporal_load(tp[j] + (int64_t)kb * (kTileBytes / 16) + lane);
+                f.wb[i][j] = __builtin_nontemporal_load(tp[j] + (int64_t)kb * (kTileBytes / 16) + 64 + lane);
+                f.ws[i][j] = wsp[j][2 * kb + (g >> 1)];
+            }
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                f.xa[i][t] = *reinterpret_cast<const uint4 *>(xp[t] + kb * HA_FP8_BLOCK);
-                f.xb[i][t] = *reinterpret_cast<const uint4 *>(xp[t] + kb * HA_FP8_BLOCK + 64);
+                f.xa[i][t] = *reinterpret_cast<const u32x4 *>(xp[t] + kb * HA_FP8_BLOCK);
+                f.xb[i][t] = *reinterpret_cast<const u32x4 *>(xp[t] + kb * HA_FP8_BLOCK + 64);
                 f.xs[i][t] = xsp[t][kb];
             }
         }
     };
-    f32x4 acc[MT];
+    f32x4 acc[NT][MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (begin < end) {
-        Group now, next;
-        fetch(now, begin);
-        for (int kb = begin; kb < end; kb += PF) {
-            if (kb + PF < end) fetch(next, kb + PF);
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < PF; ++i) {
-                if (kb + i < end) {
+        for (int t = 0; t < MT; ++t) acc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Group &f, int count) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            if (i < count) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
                     Operand<EXACT> w, v;
-                    w.take(now.wa[i], now.wb[i]);
+                    w.take(f.wa[i][j], f.wb[i][j]);
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
-                        v.take(now.xa[i][t], now.xb[i][t]);
+                        v.take(f.xa[i][t], f.xb[i][t]);
                         const f32x4 part = Operand<EXACT>::product(w, v);
-                        const float s = now.xs[i][t] * now.ws[i];
+                        const float s = f.xs[i][t] * f.ws[i][j];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(part[e], s, acc[t][e]);
+                        for (int e = 0; e < 4; ++e) acc[j][t][e] = fmaf(part[e], s, acc[j][t][e]);
                     }
                 }
             }
+        }
+    };
+    if (begin < end) {
+        Group now, next;
+        fetch(now, begin);
+        int kb = begin;
+        // the loop always requests: behind a request that may not have been made, the compiler waits for all of them
+        for (; kb + PF < end; kb += PF) {
+            fetch(next, kb + PF);
+            __builtin_amdgcn_sched_barrier(0);  // in front of the products: the compiler would move the requests behind them
+            multiply(now, PF);
             now = next;
         }
+        multiply(now, end - kb);
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_c[wave][4 * g + i][16 * t + r] = acc[t][i];
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_c[wave][16 * j + 4 * g + i][16 * t + r] = acc[j][t][i];
     __syncthreads();
-    join_waves<NWAVE, MT, GLU>(s_c, ep, nt, m0, M, N);
+    join_waves<NWAVE, NT, MT, GLU>(s_c, ep, nt, m0, M, N);
 }
 
 // ---- few rows: x in registers, the weights streamed once
@@ -319,73 +345,73 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_rows_kernel(const uint8
     const int m0 = turn % groups_m * 16 * MT, kb0 = wave * KW;
     int nt = turn / groups_m * 8 + (int)(blockIdx.x & 7);
 
+    // Tiles are requested without a condition (behind a request that may not have been made, the compiler waits for all of them):
+    // blocks beyond K are read as the last one and count nothing, rows beyond M as the last one and are not stored.
     struct Group {
-        uint4 a[PF], b[PF];
+        u32x4 a[PF], b[PF];
         float s[PF];
     };
-    auto fetch = [&](Group &w, int nt, int j0) {
-        const int64_t tile = (int64_t)nt * kb_count + kb0 + j0;
-        const uint4 *tp = reinterpret_cast<const uint4 *>(tiles + tile * kTileBytes) + lane;
-        const float *sp = ws + tile * 2 + (g >> 1);
+    auto fetch = [&](Group &w, int nt, int j0) __attribute__((always_inline)) {
+        const int64_t tile = (int64_t)nt * kb_count;
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
-            w.a[i] = w.b[i] = make_uint4(0u, 0u, 0u, 0u);
-            w.s[i] = 0.f;
-            if (nt < n_tiles && kb0 + j0 + i < kb_count) {
-                w.a[i] = ha_load16_stream(tp + i * (kTileBytes / 16));
-                w.b[i] = ha_load16_stream(tp + i * (kTileBytes / 16) + 64);
-                w.s[i] = sp[2 * i];
-            }
+            const int kb = kb0 + j0 + i, from = min(kb, kb_count - 1);
+            const u32x4 *tp = reinterpret_cast<const u32x4 *>(tiles + (tile + from) * kTileBytes) + lane;
+            w.a[i] = __builtin_nontemporal_load(tp);
+            w.b[i] = __builtin_nontemporal_load(tp + 64);
+            w.s[i] = ws[(tile + from) * 2 + (g >> 1)];
         }
     };
+    if (nt >= n_tiles) return;
     Group now, next;
     fetch(now, nt, 0);  // the first weights are on their way before x is set up
-    uint4 xa[KW][MT], xb[KW][MT];
+    u32x4 xa[KW][MT], xb[KW][MT];
     float xsc[KW][MT];
 #pragma unroll
     for (int j = 0; j < KW; ++j)
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const int m = m0 + 16 * t + r;
-            xa[j][t] = xb[j][t] = make_uint4(0u, 0u, 0u, 0u);
-            xsc[j][t] = 0.f;
-            if (m < M && kb0 + j < kb_count) {
-                const uint4 *xp = reinterpret_cast<const uint4 *>(x + m * x_sm + (kb0 + j) * HA_FP8_BLOCK + g * 16);
-                xa[j][t] = xp[0];
-                xb[j][t] = xp[4];
-                xsc[j][t] = xs[m * xs_sm + kb0 + j];
+            const int64_t m = min(m0 + 16 * t + r, M - 1);
+            const int kb = min(kb0 + j, kb_count - 1);
+            const u32x4 *xp = reinterpret_cast<const u32x4 *>(x + m * x_sm + kb * HA_FP8_BLOCK + g * 16);
+            xa[j][t] = xp[0];
+            xb[j][t] = xp[4];
+            xsc[j][t] = xs[m * xs_sm + kb];
+        }
+    f32x4 acc[MT];
+    auto multiply = [&](const Group &w, int j0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            Operand<EXACT> wo, v;
+            wo.take(w.a[i], w.b[i]);
+            const bool counts = kb0 + j0 + i < kb_count;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                v.take(xa[j0 + i][t], xb[j0 + i][t]);
+                const f32x4 part = Operand<EXACT>::product(wo, v);
+                const float s = counts ? xsc[j0 + i][t] * w.s[i] : 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(part[e], s, acc[t][e]);
             }
         }
-    while (nt < n_tiles) {
-        const int nt_next = nt + step;
+    };
+    // one tile: its first group is in `now`; the first group of `then` (if any) is there afterwards
+    auto tile = [&](int nt, int then, bool more) __attribute__((always_inline)) {
         if constexpr (EXACT && !WIDE) {  // the compiler would widen x once, in front of the loop, at twice the registers
 #pragma unroll
             for (int j = 0; j < KW; ++j)
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
-                    asm volatile("" : "+v"(xa[j][t].x), "+v"(xa[j][t].y), "+v"(xa[j][t].z), "+v"(xa[j][t].w), "+v"(xb[j][t].x),
-                                 "+v"(xb[j][t].y), "+v"(xb[j][t].z), "+v"(xb[j][t].w));
+                    asm volatile("" : "+v"(xa[j][t]), "+v"(xb[j][t]));
         }
-        f32x4 acc[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j0 = 0; j0 < KW; j0 += PF) {
             if (j0 + PF < KW) fetch(next, nt, j0 + PF);
-            else fetch(next, nt_next, 0);  // nothing is requested past the last tile
-#pragma unroll
-            for (int i = 0; i < PF; ++i) {
-                Operand<EXACT> w, v;
-                w.take(now.a[i], now.b[i]);
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    v.take(xa[j0 + i][t], xb[j0 + i][t]);
-                    const f32x4 part = Operand<EXACT>::product(w, v);
-                    const float s = xsc[j0 + i][t] * now.s[i];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(part[e], s, acc[t][e]);
-                }
-            }
+            else if (more) fetch(next, then, 0);
+            __builtin_amdgcn_sched_barrier(0);  // in front of the products: the compiler would move the requests behind them
+            multiply(now, j0);
             now = next;
         }
 #pragma unroll
@@ -393,10 +419,11 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_rows_kernel(const uint8
 #pragma unroll
             for (int i = 0; i < 4; ++i) s_c[wave][4 * g + i][16 * t + r] = acc[t][i];
         __syncthreads();
-        join_waves<NWAVE, MT, GLU>(s_c, ep, nt, m0, M, N);
-        nt = nt_next;
-        if (nt < n_tiles) __syncthreads();  // the sums are read: the next tile's may overwrite them
-    }
+        join_waves<NWAVE, 1, MT, GLU>(s_c, ep, nt, m0, M, N);
+        if (more) __syncthreads();  // the sums are read: the next tile's may overwrite them
+    };
+    for (; nt + step < n_tiles; nt += step) tile(nt, nt + step, true);
+    tile(nt, nt, false);
 }
 
 // ---- many rows: tiles of BN weight rows x BM rows of x per workgroup, staged through LDS
@@ -416,7 +443,6 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_rows_kernel(const uint8
 // for both sides, which is why targets of one call lie kStep apart.
 // Inline assembly, because the compiler would wait for all of them in front of every LDS read it cannot tell from their target;
 // the waits are written by hand (requests_arrived).  M0 holds the LDS address; nothing else in the kernel uses M0.
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x4 resource(const void *base) {  // uniform base; every access of this file is in bounds by itself
     const uint64_t b = (uint64_t)base;
     return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32)),
@@ -447,12 +473,12 @@ __device__ __forceinline__ void requests_arrived() {
     __syncthreads();
 }
 
-template <int WN, int WM, int TN, int TM, int AHEAD, bool EXACT, bool GLU>
+template <int WN, int WM, int TN, int TM, int AHEAD, bool EXACT, bool GLU, bool SPLIT>
 __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uint8_t *__restrict__ x, int64_t x_sm,
                                                                        const float *__restrict__ xs, int64_t xs_sm,
                                                                        const uint8_t *__restrict__ tiles, const float *__restrict__ ws,
                                                                        Epilogue ep, int M, int N, int kb_count, int n_tiles, int tiles_n,
-                                                                       int tiles_m, int per_xcd) {
+                                                                       int tiles_m, int per_xcd, int per_split, float *__restrict__ partial) {
     constexpr int NW = WN * WM, BN = 16 * TN * WN, BM = 16 * TM * WM, TH = TN / 2;
     constexpr int kWBytes = BN * HA_FP8_BLOCK, kXBytes = BM * HA_FP8_BLOCK, kBuffer = kWBytes + kXBytes;
     constexpr int kHalfPieces = kWBytes / 2048 / NW, kXPieces = kXBytes / 1024 / NW;  // requests per wave: half of the weights, x
@@ -463,8 +489,18 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     __shared__ float s_xs[2][BM], s_ws[2][NW * 64];
     // Workgroups go to the XCDs in turn: XCD j takes a run of tiles, four tiles of x wide and then along N, so that the 32 CUs
     // that share an L2 work on a compact block of the result.
-    const int linear = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-    if (linear >= tiles_n * tiles_m) return;
+    int linear = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3), kb_begin = 0, kb_end = kb_count;
+    int64_t split = 0;
+    if constexpr (SPLIT) {  // the splits of a tile share an XCD, one behind the other
+        const int all = tiles_n * tiles_m;
+        split = linear / all;
+        linear -= (int)split * all;
+        kb_begin = (int)split * per_split;
+        kb_end = min(kb_begin + per_split, kb_count);
+        if (kb_begin >= kb_end) return;
+    } else {
+        if (linear >= tiles_n * tiles_m) return;
+    }
     const int band = linear / (4 * tiles_n), in_band = linear - band * 4 * tiles_n, rows_in_band = min(4, tiles_m - 4 * band);
     const int bm = 4 * band + in_band % rows_in_band, bn = in_band / rows_in_band;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
@@ -491,16 +527,16 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     }
     const uint32_t xs_off = (uint32_t)min((wave % (BM / 64)) * 64 + lane, M - 1 - m0) * (uint32_t)xs_sm * 4u, ws_off = (g >> 1) * 4u;
     const uint32_t lds_buf = (uint32_t)(uintptr_t)&s_buf[0][0], lds_xs = (uint32_t)(uintptr_t)&s_xs[0][0], lds_ws = (uint32_t)(uintptr_t)&s_ws[0][0];
-    // kb: the place; from min(kb, last), so that the loop's requests (hence its waits) are the same in every turn
+    // kb: the place; from min(kb, last of the range), so that the loop's requests (hence its waits) are the same in every turn
     auto request_half = [&](int kb, int h) {
-        request16x2(w_res, w_off[h], min(kb, kb_count - 1) * kTileBytes, lds_buf + (kb & 1) * kBuffer + w_at[h]);
+        request16x2(w_res, w_off[h], min(kb, kb_end - 1) * kTileBytes, lds_buf + (kb & 1) * kBuffer + w_at[h]);
     };
     auto request_x = [&](int kb) {
-        request16x4(x_res, x_off, min(kb, kb_count - 1) * HA_FP8_BLOCK, lds_buf + (kb & 1) * kBuffer + kWBytes + wave * 4096);
+        request16x4(x_res, x_off, min(kb, kb_end - 1) * HA_FP8_BLOCK, lds_buf + (kb & 1) * kBuffer + kWBytes + wave * 4096);
     };
     auto request_scales = [&](int kb) {
-        request4(xs_res, xs_off, min(kb, kb_count - 1) * 4, lds_xs + ((kb & 1) * BM + wave % (BM / 64) * 64) * 4);
-        request4(ws_res, ws_off, min(kb, kb_count - 1) * 8, lds_ws + ((kb & 1) * NW + wave) * 256);
+        request4(xs_res, xs_off, min(kb, kb_end - 1) * 4, lds_xs + ((kb & 1) * BM + wave % (BM / 64) * 64) * 4);
+        request4(ws_res, ws_off, min(kb, kb_end - 1) * 8, lds_ws + ((kb & 1) * NW + wave) * 256);
     };
 
     f32x4 acc[TN][TM];
@@ -517,7 +553,7 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     float s[TM], s_next[TM + 1];  // of the next block as they lie in LDS: rows of x, weights
     auto load_row = [&](int kb, int u) {
         const uint8_t *b = &s_buf[0][0] + (kb & 1) * kBuffer + u * kTileBytes;
-        xo[u].take(*reinterpret_cast<const uint4 *>(b + x_first), *reinterpret_cast<const uint4 *>(b + x_second));
+        xo[u].take(*reinterpret_cast<const u32x4 *>(b + x_first), *reinterpret_cast<const u32x4 *>(b + x_second));
     };
     auto load_scales = [&](int kb) {
         s_next[TM] = s_ws[kb & 1][wave * 64 + lane];
@@ -526,27 +562,26 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     };
     auto load_weights = [&](Operand<EXACT> &w, int kb, int t) {
         const uint8_t *b = &s_buf[0][0] + (kb & 1) * kBuffer + w_first + t * kTileBytes;
-        w.take(*reinterpret_cast<const uint4 *>(b), *reinterpret_cast<const uint4 *>(b + 1024));
+        w.take(*reinterpret_cast<const u32x4 *>(b), *reinterpret_cast<const u32x4 *>(b + 1024));
     };
     static_assert(TN % kRing == 0 && kAhead < TH, "a block ends on the operand register it began with; its halves are further apart");
     // the order of requests: of every block x, scales, first half, then the second half
-    request_x(0);
-    request_scales(0);
-    request_half(0, 0);
-    request_half(0, 1);
-    request_x(1);
-    request_scales(1);
-    request_half(1, 0);
-    request_half(1, 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        request_x(kb_begin + i);
+        request_scales(kb_begin + i);
+        request_half(kb_begin + i, 0);
+        request_half(kb_begin + i, 1);
+    }
     requests_arrived<kFirst + 2 * kSecond>();
 #pragma unroll
-    for (int t = 0; t < kAhead; ++t) load_weights(wo[t], 0, t);
+    for (int t = 0; t < kAhead; ++t) load_weights(wo[t], kb_begin, t);
 #pragma unroll
-    for (int u = 0; u < TM; ++u) load_row(0, u);
-    load_scales(0);
+    for (int u = 0; u < TM; ++u) load_row(kb_begin, u);
+    load_scales(kb_begin);
     // One block of 128 inputs per turn: TN x TM matrix instructions, the multiply-adds of a tile under those of the next one, weights
     // read from LDS kAhead tiles ahead, a row of the next block's x as soon as its last instruction is issued.
-    for (int kb = 0; kb < kb_count; ++kb) {
+    for (int kb = kb_begin; kb < kb_end; ++kb) {
 #pragma unroll
         for (int u = 0; u < TM; ++u) s[u] = s_next[u] * s_next[TM];
 #pragma unroll
@@ -588,6 +623,19 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     requests_arrived<0>();
 
     // acc[t][u][i]: weight row 4 g + i of tile t, row 16 u + r of x
+    if constexpr (SPLIT) {  // the split's sums in tile order, [split][m][16 n_tiles]: join_splits finishes them
+        const int64_t width = 16LL * n_tiles;
+#pragma unroll
+        for (int u = 0; u < TM; ++u) {
+            const int m = m0 + (wm * TM + u) * 16 + r;
+            if (m >= M) continue;
+            float *row = partial + (split * M + m) * width + (nt0 + wn * TN) * 16 + 4 * g;
+#pragma unroll
+            for (int t = 0; t < TN; ++t)
+                if (nt0 + wn * TN + t < n_tiles) *reinterpret_cast<f32x4 *>(row + 16 * t) = acc[t][u];
+        }
+        return;
+    }
     constexpr int BO = GLU ? BN / 2 : BN;  // columns of out per workgroup
     const int n_out = GLU ? N / 2 : N, n0 = bn * BO;
     auto each = [&](auto put) {
@@ -643,6 +691,41 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     }
 }
 
+// Sums of the splits in their order, then residual or SwiGLU and the one rounding.  Four columns of out per thread.
+template <bool GLU>
+__global__ __launch_bounds__(256) void join_splits_kernel(const float *__restrict__ partial, int splits, Epilogue ep, int M, int N, int n_tiles) {
+    const int cols = GLU ? N / 2 : N, per_row = (cols + 3) / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t m = i / per_row, width = 16LL * n_tiles;
+    if (m >= M) return;
+    const int n = (int)(i - m * per_row) * 4, at = GLU ? (n >> 3) * 16 + (n & 7) : n;
+    const float *p = partial + m * width + at;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f}, up = y;
+    for (int s = 0; s < splits; ++s, p += (int64_t)M * width) {
+        y += *reinterpret_cast<const f32x4 *>(p);
+        if constexpr (GLU) up += *reinterpret_cast<const f32x4 *>(p + 8);
+    }
+    if constexpr (GLU) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = y[k] / (1.0f + expf(-y[k])) * up[k];
+    }
+    if (ep.out_dtype == HA_F32) {
+        store4(ep, m, n, cols, y);
+        return;
+    }
+    if (ep.res) add_residual(ep, m, n, cols, y);
+    const uint2 v = narrow4(y, ep.out_dtype);
+    uint16_t *o = (uint16_t *)ep.out + m * ep.out_sm + n;
+    if (ep.wide && n + 4 <= cols) {
+        *reinterpret_cast<uint2 *>(o) = v;
+    } else {
+        const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (n + k < cols) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+    }
+}
+
 struct Args {
     hipStream_t stream;
     const uint8_t *x;
@@ -670,15 +753,15 @@ void launch_rows(const Args &a) {
                            a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, groups);
 }
 
-template <int NWAVE, int PF, int MT, bool EXACT>
+template <int NWAVE, int PF, int NT, int MT, bool EXACT>
 void launch_stream(const Args &a) {
     const int groups = (a.M + 16 * MT - 1) / (16 * MT);
-    const unsigned grid = (unsigned)groups * (unsigned)((a.p.n_tiles + 7) / 8 * 8);
+    const unsigned grid = (unsigned)groups * (unsigned)(((a.p.n_tiles + NT - 1) / NT + 7) / 8 * 8);
     if (a.act)
-        hipLaunchKernelGGL((linear_fp8_stream_kernel<NWAVE, PF, MT, EXACT, true>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x, a.x_sm,
+        hipLaunchKernelGGL((linear_fp8_stream_kernel<NWAVE, PF, NT, MT, EXACT, true>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x, a.x_sm,
                            a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, groups);
     else
-        hipLaunchKernelGGL((linear_fp8_stream_kernel<NWAVE, PF, MT, EXACT, false>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x, a.x_sm,
+        hipLaunchKernelGGL((linear_fp8_stream_kernel<NWAVE, PF, NT, MT, EXACT, false>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x, a.x_sm,
                            a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, groups);
 }
 
@@ -687,22 +770,58 @@ void launch_tiled(const Args &a) {
     const int tiles_n = (a.p.n_tiles + WN * TN - 1) / (WN * TN), tiles_m = (a.M + 16 * WM * TM - 1) / (16 * WM * TM);
     const int per_xcd = (int)(((int64_t)tiles_n * tiles_m + 7) / 8);
     if (a.act)
-        hipLaunchKernelGGL((linear_fp8_tiled_kernel<WN, WM, TN, TM, AHEAD, EXACT, true>), dim3(8u * (unsigned)per_xcd), dim3(WN * WM * 64), 0,
-                           a.stream, a.x, a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, tiles_n, tiles_m, per_xcd);
+        hipLaunchKernelGGL((linear_fp8_tiled_kernel<WN, WM, TN, TM, AHEAD, EXACT, true, false>), dim3(8u * (unsigned)per_xcd), dim3(WN * WM * 64),
+                           0, a.stream, a.x, a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, tiles_n, tiles_m, per_xcd,
+                           a.p.kb, nullptr);
     else
-        hipLaunchKernelGGL((linear_fp8_tiled_kernel<WN, WM, TN, TM, AHEAD, EXACT, false>), dim3(8u * (unsigned)per_xcd), dim3(WN * WM * 64), 0,
-                           a.stream, a.x, a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, tiles_n, tiles_m, per_xcd);
+        hipLaunchKernelGGL((linear_fp8_tiled_kernel<WN, WM, TN, TM, AHEAD, EXACT, false, false>), dim3(8u * (unsigned)per_xcd), dim3(WN * WM * 64),
+                           0, a.stream, a.x, a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, tiles_n, tiles_m, per_xcd,
+                           a.p.kb, nullptr);
 }
 
-// 17 to 128 rows (and more where tiles do not apply)
+// Whether x of 17 to 128 rows stays in registers, weights streamed past it: rows of 16 to 32 blocks.  Against tiles with K cut
+// (6144 x 4096): 32 rows 11.4 us (13.7), 64 rows 17.4 (15.7), 128 rows 19.3 (19.7); of few tiles (1024 x 4096) only up to 32 rows: 9.1
+// us (10.2), 64 rows 14.6 (11.0).
+bool keeps_rows(int M, Packed p) { return M <= 128 && p.kb >= 16 && p.kb <= 32 && (M <= 32 || p.n_tiles > 128); }
+
+// How many ways K is cut for tiles of 128 x 128: into as many as give every CU a tile, of at least four blocks (cut for two
+// tiles per CU instead, the longer sum of the parts costs more than it brings: 4096 x 14336, 256 rows 41 us against 37; not cut 96).
+struct Splits {
+    int count, per;
+};
+Splits splits_for(int M, Packed p) {
+    if (M <= 16 || p.kb < 8 || keeps_rows(M, p)) return {1, p.kb};
+    const int64_t tiles = ((p.n_tiles + 7LL) / 8) * ((M + 127LL) / 128);
+    int64_t want = 256 / tiles;
+    if (want > p.kb / 4) want = p.kb / 4;
+    if (want < 2) return {1, p.kb};
+    const int per = (int)((p.kb + want - 1) / want);
+    return {(p.kb + per - 1) / per, per};
+}
+
+template <bool EXACT>
+void launch_split(const Args &a, Splits s, float *partial) {
+    const int tiles_n = (a.p.n_tiles + 7) / 8, tiles_m = (a.M + 127) / 128;
+    const int per_xcd = (int)(((int64_t)tiles_n * tiles_m * s.count + 7) / 8);
+    hipLaunchKernelGGL((linear_fp8_tiled_kernel<2, 2, 4, 4, 1, EXACT, false, true>), dim3(8u * (unsigned)per_xcd), dim3(256), 0, a.stream, a.x,
+                       a.x_sm, a.xs, a.xs_sm, a.tiles, a.ws, a.ep, a.M, a.N, a.p.kb, a.p.n_tiles, tiles_n, tiles_m, per_xcd, s.per, partial);
+    const int cols = a.act ? a.N / 2 : a.N;
+    const unsigned grid = (unsigned)(((int64_t)a.M * ((cols + 3) / 4) + 255) / 256);
+    if (a.act)
+        hipLaunchKernelGGL(join_splits_kernel<true>, dim3(grid), dim3(256), 0, a.stream, partial, s.count, a.ep, a.M, a.N, a.p.n_tiles);
+    else
+        hipLaunchKernelGGL(join_splits_kernel<false>, dim3(grid), dim3(256), 0, a.stream, partial, s.count, a.ep, a.M, a.N, a.p.n_tiles);
+}
+
+// 17 rows and more without tiles
 template <bool EXACT>
 void launch_some_rows(const Args &a) {
-    if (a.p.kb <= 32) {
+    if (keeps_rows(a.M, a.p)) {
         if (a.M <= 32) launch_rows<8, 4, 4, 2, false, EXACT>(a);
         else launch_rows<8, 4, 2, 4, false, EXACT>(a);
     } else {
-        if (a.M <= 32) launch_stream<8, 2, 2, EXACT>(a);
-        else launch_stream<8, 2, 4, EXACT>(a);
+        if (a.M <= 32) launch_stream<8, 2, 2, 2, EXACT>(a);
+        else launch_stream<8, 1, 2, 4, EXACT>(a);
     }
 }
 
@@ -714,6 +833,13 @@ int64_t ha_weight_fp8_bytes(int N, int K, int glu) {
     if (N < 1 || K < 1 || (glu && N % 2 != 0)) return 0;
     const Packed p = packed_shape(N, K, glu);
     return (int64_t)p.n_tiles * p.kb * kTileBytes;
+}
+
+size_t ha_linear_fp8_workspace_bytes(int M, int N, int K, int act) {
+    if (M < 1 || ha_weight_fp8_bytes(N, K, act) == 0) return 0;
+    const Packed p = packed_shape(N, K, act);
+    const Splits s = splits_for(M, p);
+    return s.count > 1 ? (size_t)s.count * (size_t)M * 16u * (size_t)p.n_tiles * sizeof(float) : 0;
 }
 
 int64_t ha_weight_fp8_scales(int N, int K, int glu) { return ha_weight_fp8_bytes(N, K, glu) / kTileBytes * 2; }
@@ -743,7 +869,7 @@ int ha_pack_weight_fp8(const void *w, int64_t w_stride_n, int dtype, const float
 
 int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, int64_t x_scales_stride_m, const void *tiles,
                   const float *tile_scales, const void *residual, int64_t residual_stride_m, int act, void *out, int64_t out_stride_m,
-                  int out_dtype, int M, int N, int K, void *stream) {
+                  int out_dtype, int M, int N, int K, void *workspace, size_t workspace_bytes, void *stream) {
     HA_REQUIRE(tiles && tile_scales && (M == 0 || (xq && x_scales && out)), HA_ERR_NULL_POINTER,
                "xq/x_scales/tiles/tile_scales/out is NULL");
     HA_REQUIRE(out_dtype == HA_F32 || out_dtype == HA_BF16 || out_dtype == HA_F16, HA_ERR_BAD_DTYPE, "unknown dtype %d", out_dtype);
@@ -760,8 +886,7 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
                "rows of xq and tiles must be 16-byte aligned");
     HA_REQUIRE(ha_aligned(x_scales, 4) && ha_aligned(tile_scales, 8) && ha_aligned(out, es) && ha_aligned(residual, es), HA_ERR_MISALIGNED,
                "pointers are not aligned to their elements");
-    int st = ha_require_device();
-    if (st || M == 0) return st;
+    int st;
     const bool wide = ha_aligned(out, 4 * es) && out_stride_m % 4 == 0 && (!residual || (ha_aligned(residual, 4 * es) && residual_stride_m % 4 == 0));
     const Epilogue ep = {residual, residual_stride_m, out, out_stride_m, out_dtype, wide, ha_aligned(out, 8 * es) && out_stride_m % 8 == 0};
     const Args a = {(hipStream_t)stream, (const uint8_t *)xq, xq_stride_m, x_scales, x_scales_stride_m, (const uint8_t *)tiles, tile_scales, ep,
@@ -769,8 +894,19 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
     const bool exact = out_dtype == HA_F32;
     HA_REQUIRE(((int64_t)M + 15) / 16 * (p.n_tiles + 7LL) <= 2147483647LL, HA_ERR_BAD_SHAPE, "too many tiles for one launch");
     // offsets within a workgroup's tiles are 32-bit
-    const bool tiled = M > 128 && 256 * (xq_stride_m + x_scales_stride_m * 4) < (1LL << 31) && (int64_t)p.kb * kTileBytes * 16 < (1LL << 31);
-    if (tiled) {
+    const bool in_reach = 256 * (xq_stride_m + x_scales_stride_m * 4) < (1LL << 31) && (int64_t)p.kb * kTileBytes * 16 < (1LL << 31);
+    const Splits splits = in_reach ? splits_for(M, p) : Splits{1, p.kb};
+    if (splits.count > 1) {
+        const size_t need = ha_linear_fp8_workspace_bytes(M, N, K, act);
+        HA_REQUIRE(workspace && workspace_bytes >= need, HA_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+        HA_REQUIRE(ha_aligned(workspace, 16), HA_ERR_MISALIGNED, "workspace must be 16-byte aligned");
+    }
+    st = ha_require_device();
+    if (st || M == 0) return st;
+    if (splits.count > 1) {
+        if (exact) launch_split<true>(a, splits, (float *)workspace);
+        else launch_split<false>(a, splits, (float *)workspace);
+    } else if (in_reach && M > 128) {
         const int64_t big = ((p.n_tiles + 15LL) / 16) * ((M + 255LL) / 256);
         if (exact) launch_tiled<2, 2, 4, 4, 1, true>(a);
         else if (big >= 200) launch_tiled<2, 4, 8, 4, 3, false>(a);
@@ -780,7 +916,7 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
         else if (p.kb <= 16) launch_rows<8, 2, 2, 1, true, true>(a);
         else if (p.kb <= 32 && p.n_tiles < 1024) launch_rows<8, 4, 4, 1, true, true>(a);
         else if (p.kb <= 32) launch_rows<8, 4, 2, 1, false, true, 2>(a);
-        else launch_stream<16, 2, 1, true>(a);
+        else launch_stream<16, 2, 1, 1, true>(a);
     } else if (exact) {
         launch_some_rows<true>(a);
     } else {

@@ -161,7 +161,9 @@ def _declare(lib: C.CDLL) -> C.CDLL:
     lib.ha_pack_weight_fp8.restype = i32
     lib.ha_pack_weight_fp8.argtypes = [vp, i64, i32, vp, i64, i32, i32, i32, vp, vp, vp]
     lib.ha_linear_fp8.restype = i32
-    lib.ha_linear_fp8.argtypes = [vp, i64, vp, i64, vp, vp, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp]
+    lib.ha_linear_fp8.argtypes = [vp, i64, vp, i64, vp, vp, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp, sz, vp]
+    lib.ha_linear_fp8_workspace_bytes.restype = sz
+    lib.ha_linear_fp8_workspace_bytes.argtypes = [i32, i32, i32, i32]
     lib.ha_window_partial_bytes.restype = sz
     lib.ha_window_partial_bytes.argtypes = [i32, i32]
     lib.ha_window_partial.restype = i32
@@ -910,10 +912,18 @@ def pack_weight_fp8(w: torch.Tensor, scales: Optional[torch.Tensor] = None, glu:
     return out
 
 
+LINEAR_FP8_UNSPLIT_ROWS = 16     # up to this many rows no workspace is needed
+
+
+def linear_fp8_workspace_bytes(m: int, weight: Fp8Weight) -> int:
+    return load_library().ha_linear_fp8_workspace_bytes(m, weight.N, weight.K, int(weight.glu))
+
+
 def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: torch.Tensor, residual: Optional[torch.Tensor] = None,
-               swiglu: bool = False) -> torch.Tensor:
+               swiglu: bool = False, ws: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out [M, N] = rows in 8 bits (q, scales) . W^T (+ residual), or [M, N / 2] = silu(gate) * up with swiglu (weights packed with
-    glu); out fp32, bf16 or fp16, rounded once.  residual may be out itself."""
+    glu); out fp32, bf16 or fp16, rounded once.  residual may be out itself.  ws: scratch of `linear_fp8_workspace_bytes` bytes,
+    taken from torch's allocator where it is needed and not given."""
     tiles, tile_scales, n, k, glu = weight
     dev = _same_device(q, scales, tiles, tile_scales, out, residual)
     m = q.shape[0]
@@ -926,7 +936,14 @@ def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: to
         if swiglu:
             raise ValueError("SwiGLU takes no residual")
         r, r_sm = residual.data_ptr(), _rows_of(residual, "residual", m, n, out.dtype)
-    _launch_on(dev, (_lib or load_library()).ha_linear_fp8, "ha_linear_fp8",
+    lib = _lib or load_library()
+    if ws is None and m > LINEAR_FP8_UNSPLIT_ROWS:
+        nbytes = lib.ha_linear_fp8_workspace_bytes(m, n, k, 1 if swiglu else 0)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
+    elif ws is not None:
+        _same_device(out, ws)
+    _launch_on(dev, lib.ha_linear_fp8, "ha_linear_fp8",
                (q.data_ptr(), q_sm, scales.data_ptr(), s_sm, tiles.data_ptr(), tile_scales.data_ptr(), r, r_sm, 1 if swiglu else 0,
-                out.data_ptr(), o_sm, _DTYPE[out.dtype], m, n, k))
+                out.data_ptr(), o_sm, _DTYPE[out.dtype], m, n, k, None if ws is None else ws.data_ptr(),
+                0 if ws is None else ws.numel() * ws.element_size()))
     return out

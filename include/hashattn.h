@@ -530,7 +530,9 @@ int ha_linear_tiled(const void *x, int64_t x_stride_m, const void *tiles, const 
  * out [M, N / 2] = silu(gate) * up.  Products exact, sums in fp32, ONE rounding to out_dtype at the end (residual and SwiGLU before
  * it).  16-bit results of more than 16 rows are summed by the 8-bit matrix instructions, which drop what lies more than 13 bits
  * below the largest of eight neighbouring products: about 1.5e-5 of the result, where the result's own rounding is 2^-9 or 2^-12 of
- * it.  Any M, N, K; `residual` may be `out` itself.  Which kernel runs depends on the sizes, out_dtype and strides alone; a row's
+ * it.  Where a matrix has too few tiles to fill the GPU, K is cut and the parts' sums go through the workspace, in two launches:
+ * ha_linear_fp8_workspace_bytes(M, N, K, act) bytes, 16-byte aligned (0 for most sizes: NULL will do); calls that share one must
+ * not overlap.  Any M, N, K; `residual` may be `out` itself.  Which kernel runs depends on the sizes, out_dtype and strides alone; a row's
  * outputs do not depend on the other rows' values.
  */
 #define HA_FP8_BLOCK 128
@@ -547,9 +549,10 @@ int64_t ha_weight_fp8_bytes(int N, int K, int glu);
 int64_t ha_weight_fp8_scales(int N, int K, int glu);
 int ha_pack_weight_fp8(const void *w, int64_t w_stride_n, int dtype, const float *w_scales, int64_t w_scales_stride_n, int N, int K, int glu,
                        void *tiles, float *tile_scales, void *stream);
+size_t ha_linear_fp8_workspace_bytes(int M, int N, int K, int act);
 int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, int64_t x_scales_stride_m, const void *tiles,
                   const float *tile_scales, const void *residual, int64_t residual_stride_m, int act, void *out, int64_t out_stride_m,
-                  int out_dtype, int M, int N, int K, void *stream);
+                  int out_dtype, int M, int N, int K, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

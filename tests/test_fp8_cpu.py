@@ -8,7 +8,7 @@ import torch
 from hashattention import _ops
 from tests import fp8_util as ref
 
-NULL, SHAPE, DTYPE, ALIGN, NODEV = -1, -2, -3, -4, -6
+NULL, SHAPE, DTYPE, ALIGN, WS, NODEV = -1, -2, -3, -4, -5, -6
 BF16, F32, E4M3 = _ops.HA_BF16, _ops.HA_F32, _ops.HA_FP8_E4M3
 
 
@@ -73,8 +73,8 @@ def test_pack_and_linear_refuse(lib, mem):
     assert pack(dt=E4M3, ws=mem, wss=1) == SHAPE and pack(N=2 ** 31 - 1) == SHAPE
     assert pack(w=mem + 1) == ALIGN and pack(t=mem + 8) == ALIGN and pack(ts=mem + 4) == ALIGN
 
-    def lin(x=mem, xs=256, s=mem, ss=2, t=mem, ts=mem, r=None, rs=0, act=0, o=mem, os=32, dt=BF16, M=4, N=32, K=256):
-        return lib.ha_linear_fp8(x, xs, s, ss, t, ts, r, rs, act, o, os, dt, M, N, K, None)
+    def lin(x=mem, xs=256, s=mem, ss=2, t=mem, ts=mem, r=None, rs=0, act=0, o=mem, os=32, dt=BF16, M=4, N=32, K=256, ws=None, wsb=0):
+        return lib.ha_linear_fp8(x, xs, s, ss, t, ts, r, rs, act, o, os, dt, M, N, K, ws, wsb, None)
 
     for k in ("x", "s", "t", "ts", "o"):
         assert lin(**{k: None}) == NULL
@@ -83,8 +83,18 @@ def test_pack_and_linear_refuse(lib, mem):
     assert lin(act=1, r=mem, rs=32) == SHAPE and lin(xs=255) == SHAPE and lin(ss=1) == SHAPE and lin(os=31) == SHAPE and lin(r=mem, rs=31) == SHAPE
     assert lin(x=mem + 8) == ALIGN and lin(xs=264) == ALIGN and lin(t=mem + 8) == ALIGN and lin(ts=mem + 4) == ALIGN
     assert lin(s=mem + 2) == ALIGN and lin(o=mem + 1) == ALIGN and lin(r=mem + 1, rs=32) == ALIGN
+    assert lin(M=2 ** 31 - 1, N=2 ** 31 - 1, os=2 ** 31) == SHAPE
+    # sizes whose sums go through a workspace: missing, too small, misaligned
+    big = dict(M=300, N=32, K=4096, xs=4096, ss=32)
+    need = lib.ha_linear_fp8_workspace_bytes(300, 32, 4096, 0)
+    assert need == 8 * 300 * 32 * 4
+    assert lin(**big) == WS and lin(**big, ws=mem, wsb=need - 1) == WS and lin(**big, ws=mem + 8, wsb=need) == ALIGN
+    for m, n, k, act in ((4, 32, 4096, 0), (16, 4096, 14336, 0), (64, 6144, 4096, 0), (4096, 28672, 4096, 0), (0, 32, 4096, 0), (300, 33, 4096, 1)):
+        assert lib.ha_linear_fp8_workspace_bytes(m, n, k, act) == 0
+    assert lib.ha_linear_fp8_workspace_bytes(300, 33, 4096, 0) > 0
+    assert _ops.LINEAR_FP8_UNSPLIT_ROWS == 16 and lib.ha_linear_fp8_workspace_bytes(17, 32, 14336, 0) > 0
     if lib.ha_device_count() == 0:
-        assert pack() == NODEV and lin() == NODEV
+        assert pack() == NODEV and lin() == NODEV and lin(**big, ws=mem, wsb=need) == NODEV
 
 
 def test_bindings_take_gpu_tensors_only():

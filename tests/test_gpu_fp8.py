@@ -206,7 +206,9 @@ def eight_bit_sums(m, out_dtype):
 
 LINEAR_SIZES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (4, 6144, 4096), (4, 4096, 14336), (15, 100, 300), (16, 256, 1111), (17, 130, 257),
                 (31, 48, 1000), (33, 1000, 127), (64, 512, 4096), (65, 257, 640), (100, 1000, 1111), (128, 512, 1024), (200, 640, 384),
-                (256, 256, 2048), (300, 129, 2000), (513, 384, 512), (1000, 1030, 900), (2048, 1024, 512)]
+                (256, 256, 2048), (300, 129, 2000), (513, 384, 512), (1000, 1030, 900), (2048, 1024, 512),
+                (20, 130, 4200), (40, 300, 14336), (90, 1000, 2200), (130, 2000, 4000), (257, 700, 1100), (700, 3000, 640),
+                (3000, 5000, 300)]
 
 
 @pytest.mark.parametrize("out_dtype", DTYPES)
@@ -221,7 +223,8 @@ def test_linear(m, n, k, out_dtype):
     assert torch.equal(_ops.linear_fp8(q, s, w, again), out), "the same bits on every run"
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 33, 100), (4, 4096, 1024), (20, 200, 300), (48, 300, 1111), (130, 384, 640), (512, 512, 256), (700, 1000, 384)])
+@pytest.mark.parametrize("m,n,k", [(1, 33, 100), (4, 4096, 1024), (20, 200, 300), (48, 300, 1111), (130, 384, 640), (512, 512, 256), (700, 1000, 384),
+                                   (50, 260, 4300), (300, 515, 1200), (2100, 6000, 200)])
 @pytest.mark.parametrize("out_dtype", DTYPES)
 def test_linear_residual(m, n, k, out_dtype):
     q, s, wq, ws = make_linear(m, n, k, seed=1)
@@ -236,7 +239,7 @@ def test_linear_residual(m, n, k, out_dtype):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 2, 128), (4, 28672, 512), (16, 2 * 37, 300), (17, 2 * 130, 257), (40, 2 * 200, 1000), (129, 2 * 256, 384),
-                                   (520, 2 * 384, 256), (600, 2 * 333, 500)])
+                                   (520, 2 * 384, 256), (600, 2 * 333, 500), (60, 2 * 1001, 4096), (150, 2 * 515, 1500), (2100, 2 * 3001, 200)])
 @pytest.mark.parametrize("out_dtype", DTYPES)
 def test_linear_swiglu(m, n, k, out_dtype):
     q, s, wq, ws = make_linear(m, n, k, seed=3, glu=True)
@@ -333,6 +336,22 @@ def test_packing_takes_numbers_and_scales_over_as_they_are():
     w = _ops.pack_weight_fp8(wide[:, 3:k + 3].view(torch.float8_e4m3fn), scales=ws)
     out = _ops.linear_fp8(q, s, w, torch.empty(4, n, device=DEV))
     ref.assert_linear(out, *ref.linear(q, s, wq, ws, k))
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 300, 4300), (300, 512, 2048)])
+def test_linear_with_a_workspace_of_the_callers(m, n, k):
+    """The same bits from the caller's scratch as from the allocator's; what lies behind the bytes asked for stays; too little is refused."""
+    q, s, wq, ws = make_linear(m, n, k, seed=21)
+    w = _ops.pack_weight_fp8(wq, scales=ws)
+    need = _ops.linear_fp8_workspace_bytes(m, w)
+    assert need > 0
+    mem = torch.full((need + 256,), 0x5a, dtype=torch.uint8, device=DEV)
+    a = _ops.linear_fp8(q, s, w, torch.empty(m, n, dtype=torch.bfloat16, device=DEV))
+    b = _ops.linear_fp8(q, s, w, torch.empty(m, n, dtype=torch.bfloat16, device=DEV), ws=mem[:need])
+    assert torch.equal(a, b) and (mem[need:] == 0x5a).all()
+    ref.assert_linear(a, *ref.linear(q, s, wq, ws, k, eight_bit_sums=True))
+    with pytest.raises(_ops.HashAttnError):
+        _ops.linear_fp8(q, s, w, b, ws=mem[:need - 16])
 
 
 def test_no_rows_is_no_work():
