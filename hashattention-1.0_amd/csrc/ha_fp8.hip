@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void rows_fp8_kernel(const char *__restrict__ 
         float u[8];
         load8_guarded<E, VEC>(row + (int64_t)K * Elem<E>::bytes, k0, K, u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] / (1.0f + expf(-y[i])) * u[i];
+        for (int i = 0; i < 8; ++i) y[i] = ha_silu(y[i]) * u[i];
     }
     write_block(y, sub, q + m * q_sm + k0, scales + m * s_sm + kb);
 }

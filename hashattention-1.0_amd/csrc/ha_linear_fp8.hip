@@ -209,7 +209,7 @@ __device__ __forceinline__ void join_waves(const float (&s_c)[NWAVE][16 * NT][16
             if (m0 + mm >= M || col >= N / 2) continue;
             const int row = (c >> 3) * 16 + (c & 7);
             const float gate = total(row, mm);
-            ha_store_elem(ep.out, (m0 + mm) * ep.out_sm + col, gate / (1.0f + expf(-gate)) * total(row + 8, mm), ep.out_dtype);
+            ha_store_elem(ep.out, (m0 + mm) * ep.out_sm + col, ha_silu(gate) * total(row + 8, mm), ep.out_dtype);
         }
     } else {
         for (int t = tid; t < 16 * NT * 16 * MT; t += NWAVE * 64) {
@@ -454,12 +454,12 @@ __device__ __forceinline__ void request16x2(u32x4 res, uint32_t offset, uint32_t
                  ::"v"(offset), "s"(res), "s"(lds), "s"(from)
                  : "memory");
 }
-__device__ __forceinline__ void request16x4(u32x4 res, const uint32_t (&offset)[4], uint32_t from, uint32_t lds) {  // kStep 1024
-    asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %4, %6 offen lds\n\t"
-                 "buffer_load_dwordx4 %1, %4, %6 offen offset:1024 lds\n\t"
-                 "buffer_load_dwordx4 %2, %4, %6 offen offset:2048 lds\n\t"
-                 "buffer_load_dwordx4 %3, %4, %6 offen offset:3072 lds"
-                 ::"v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3]), "s"(res), "s"(lds), "s"(from)
+// the same with an offset of its own for each of the two, of which the first lies `first` behind lds
+template <int FIRST>
+__device__ __forceinline__ void request16_pair(u32x4 res, uint32_t offset0, uint32_t offset1, uint32_t from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, %4 offen offset:%5 lds\n\t"
+                 "buffer_load_dwordx4 %1, %2, %4 offen offset:%6 lds"
+                 ::"v"(offset0), "v"(offset1), "s"(res), "s"(lds), "s"(from), "n"(FIRST), "n"(FIRST + 1024)
                  : "memory");
 }
 __device__ __forceinline__ void request4(u32x4 res, uint32_t offset, uint32_t from, uint32_t lds) {
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     const int m0 = bm * BM, nt0 = bn * (BN / 16);
 
     // rows and tiles beyond the matrices are read as their last ones; what they give is not stored
-    static_assert(kXPieces == 4 && kHalfPieces == 2, "requests are made by four and by two");
+    static_assert(kXPieces == 4 && kHalfPieces == 2, "requests are made by two");
     const u32x4 x_res = resource(x + (int64_t)m0 * x_sm - 4096), xs_res = resource(xs + (int64_t)m0 * xs_sm);
     const u32x4 w_res = resource(tiles + (int64_t)nt0 * kb_count * kTileBytes);
     // all tiles of a wave lie in one block of 128 weight rows (glu: one of gate and one of up): one scale per lane and block of K
@@ -531,8 +531,11 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     auto request_half = [&](int kb, int h) {
         request16x2(w_res, w_off[h], min(kb, kb_end - 1) * kTileBytes, lds_buf + (kb & 1) * kBuffer + w_at[h]);
     };
-    auto request_x = [&](int kb) {
-        request16x4(x_res, x_off, min(kb, kb_end - 1) * HA_FP8_BLOCK, lds_buf + (kb & 1) * kBuffer + kWBytes + wave * 4096);
+    auto request_x0 = [&](int kb) {
+        request16_pair<0>(x_res, x_off[0], x_off[1], min(kb, kb_end - 1) * HA_FP8_BLOCK, lds_buf + (kb & 1) * kBuffer + kWBytes + wave * 4096);
+    };
+    auto request_x1 = [&](int kb) {
+        request16_pair<2048>(x_res, x_off[2], x_off[3], min(kb, kb_end - 1) * HA_FP8_BLOCK, lds_buf + (kb & 1) * kBuffer + kWBytes + wave * 4096);
     };
     auto request_scales = [&](int kb) {
         request4(xs_res, xs_off, min(kb, kb_end - 1) * 4, lds_xs + ((kb & 1) * BM + wave % (BM / 64) * 64) * 4);
@@ -548,6 +551,10 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     const uint32_t x_first = kWBytes + (wm * TM * 16 + r) * HA_FP8_BLOCK + ((g ^ r) & 7) * 16, x_second = x_first ^ 64;
     const uint32_t w_first = wn * TN * kTileBytes + lane * 16;
     constexpr int kAhead = AHEAD, kRing = kAhead + 1;  // tiles of weights read ahead of the one in use
+    // The tiles at which a block's requests are made: spread out (all of them right behind the barrier, from all waves at once,
+    // 4096 x 28672 x 4096 took 579 us against 550).
+    constexpr int kX1 = TN == 8 ? 3 : 1, kScales = TN == 8 ? 4 : 2, kHalf0 = TN == 8 ? 5 : 2;
+    static_assert(TH - kAhead <= kX1 && kX1 <= kScales && kScales <= kHalf0 && kHalf0 <= TN - kAhead, "the order that the waits count on");
     Operand<EXACT> xo[TM], wo[kRing];
     f32x4 part[2][TM];
     float s[TM], s_next[TM + 1];  // of the next block as they lie in LDS: rows of x, weights
@@ -568,7 +575,8 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
     // the order of requests: of every block x, scales, first half, then the second half
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        request_x(kb_begin + i);
+        request_x0(kb_begin + i);
+        request_x1(kb_begin + i);
         request_scales(kb_begin + i);
         request_half(kb_begin + i, 0);
         request_half(kb_begin + i, 1);
@@ -590,17 +598,14 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
                 // every wave has x and the first half of this block's weights in registers: the block after next takes their
                 // place.  Arrived: the second half of this block.
                 requests_arrived<kFirst + kSecond>();
-                request_x(kb + 2);
+                request_x0(kb + 2);
             }
-            if (t == TH - kAhead + 1) {
-                request_scales(kb + 2);
-                request_half(kb + 2, 0);
-            }
-            if (t == TN - kAhead) {
-                // every wave has the second half in registers too.  Arrived: x and the first half of the next block.
-                requests_arrived<kFirst + kSecond>();
-                request_half(kb + 2, 1);
-            }
+            if (t == kX1) request_x1(kb + 2);
+            if (t == kScales) request_scales(kb + 2);
+            if (t == kHalf0) request_half(kb + 2, 0);
+            // every wave has the second half in registers too.  Arrived: x and the first half of the next block.
+            if (t == TN - kAhead) requests_arrived<kFirst + kSecond>();
+            if (t == TN - 1) request_half(kb + 2, 1);
             if (t + kAhead < TN) load_weights(wo[(t + kAhead) % kRing], kb, t + kAhead);
             else load_weights(wo[(t + kAhead) % kRing], kb + 1, t + kAhead - TN);
             if (t == TN - 1) load_scales(kb + 1);
@@ -649,7 +654,7 @@ __global__ __launch_bounds__(WN *WM * 64) void linear_fp8_tiled_kernel(const uin
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float up = __shfl_xor(acc[t][u][i], 32);
-                        y[i] = acc[t][u][i] / (1.0f + expf(-acc[t][u][i])) * up;
+                        y[i] = ha_silu(acc[t][u][i]) * up;
                     }
                     col = (wn * TN + t) * 8 + 4 * g;
                     if (g >= 2) continue;
@@ -707,7 +712,7 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const float *__restric
     }
     if constexpr (GLU) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = y[k] / (1.0f + expf(-y[k])) * up[k];
+        for (int k = 0; k < 4; ++k) y[k] = ha_silu(y[k]) * up[k];
     }
     if (ep.out_dtype == HA_F32) {
         store4(ep, m, n, cols, y);
@@ -739,11 +744,12 @@ struct Args {
     Packed p;
 };
 
-// One workgroup per CU (PER_CU of them), in as even a number of tiles as it goes, in whole runs of 8 (the XCDs) per group of rows
-template <int NWAVE, int KW, int PF, int MT, bool WIDE, bool EXACT, int PER_CU = 1>
+// One workgroup per CU (two of them, with x not widened to make room: 28672 x 4096, 16 rows 24.3 us against 22.6), in as even a number
+// of tiles as it goes, in whole runs of 8 (the XCDs) per group of rows
+template <int NWAVE, int KW, int PF, int MT, bool WIDE, bool EXACT>
 void launch_rows(const Args &a) {
     const int groups = (a.M + 16 * MT - 1) / (16 * MT);
-    const int rounds = (int)(((int64_t)a.p.n_tiles * groups + 256 * PER_CU - 1) / (256 * PER_CU));
+    const int rounds = (int)(((int64_t)a.p.n_tiles * groups + 255) / 256);
     const unsigned grid = (unsigned)groups * (unsigned)(((a.p.n_tiles + rounds - 1) / rounds + 7) / 8 * 8);
     if (a.act)
         hipLaunchKernelGGL((linear_fp8_rows_kernel<NWAVE, KW, PF, MT, WIDE, EXACT, true>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x,
@@ -784,13 +790,17 @@ void launch_tiled(const Args &a) {
 // us (10.2), 64 rows 14.6 (11.0).
 bool keeps_rows(int M, Packed p) { return M <= 128 && p.kb >= 16 && p.kb <= 32 && (M <= 32 || p.n_tiles > 128); }
 
+// Whether a product of short rows is too small for tiles: 64 rows of x and 32 of weights per workgroup straight from memory, while
+// that is two workgroups per CU at most (2048 x 512: 256 rows 5.3 us against 9.2, 512 rows 8.7 against 9.4, 1024 rows 11.8 against 9.6).
+bool short_rows(int M, Packed p) { return p.kb <= 16 && ((M + 63LL) / 64) * ((p.n_tiles + 1LL) / 2) <= 512; }
+
 // How many ways K is cut for tiles of 128 x 128: into as many as give every CU a tile, of at least four blocks (cut for two
 // tiles per CU instead, the longer sum of the parts costs more than it brings: 4096 x 14336, 256 rows 41 us against 37; not cut 96).
 struct Splits {
     int count, per;
 };
 Splits splits_for(int M, Packed p) {
-    if (M <= 16 || p.kb < 8 || keeps_rows(M, p)) return {1, p.kb};
+    if (M <= 16 || p.kb < 8 || keeps_rows(M, p) || short_rows(M, p)) return {1, p.kb};
     const int64_t tiles = ((p.n_tiles + 7LL) / 8) * ((M + 127LL) / 128);
     int64_t want = 256 / tiles;
     if (want > p.kb / 4) want = p.kb / 4;
@@ -906,7 +916,7 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
     if (splits.count > 1) {
         if (exact) launch_split<true>(a, splits, (float *)workspace);
         else launch_split<false>(a, splits, (float *)workspace);
-    } else if (in_reach && M > 128) {
+    } else if (in_reach && M > 128 && !short_rows(M, p)) {
         const int64_t big = ((p.n_tiles + 15LL) / 16) * ((M + 255LL) / 256);
         if (exact) launch_tiled<2, 2, 4, 4, 1, true>(a);
         else if (big >= 200) launch_tiled<2, 4, 8, 4, 3, false>(a);
@@ -914,8 +924,7 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
     } else if (M <= 16) {
         if (p.kb <= 8) launch_rows<8, 1, 1, 1, true, true>(a);
         else if (p.kb <= 16) launch_rows<8, 2, 2, 1, true, true>(a);
-        else if (p.kb <= 32 && p.n_tiles < 1024) launch_rows<8, 4, 4, 1, true, true>(a);
-        else if (p.kb <= 32) launch_rows<8, 4, 2, 1, false, true, 2>(a);
+        else if (p.kb <= 32) launch_rows<8, 4, 2, 1, true, true>(a);
         else launch_stream<16, 2, 1, 1, true>(a);
     } else if (exact) {
         launch_some_rows<true>(a);
