@@ -465,11 +465,16 @@ __device__ __forceinline__ void request16_pair(u32x4 res, uint32_t offset0, uint
 __device__ __forceinline__ void request4(u32x4 res, uint32_t offset, uint32_t from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %3 offen lds" ::"v"(offset), "s"(res), "s"(lds), "s"(from) : "memory");
 }
-// Waits until at most `younger` of the wave's requests are outstanding (they arrive in the order they were made) and every wave
-// has come here; all LDS reads of the wave have arrived too.
+// Waits until at most YOUNGER of the wave's requests are outstanding (they arrive in the order they were made) and every wave
+// has come here; all LDS reads of the wave have arrived too.  The count relies on the loop having no other vector memory access:
+// no global load and no spilled register.  -DHASHATTN_STAGE_WAIT_ALL builds the conservative form, which must give the same bits.
 template <int YOUNGER>
 __device__ __forceinline__ void requests_arrived() {
+#ifdef HASHATTN_STAGE_WAIT_ALL
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#else
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(YOUNGER) : "memory");
+#endif
     __syncthreads();
 }
 

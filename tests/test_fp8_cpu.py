@@ -1,6 +1,9 @@
 """Host side of the 8-bit entry points, without a GPU: sizes, and refusals before any device work (host buffers stand in for device
 pointers; nothing is launched).  The 64-bit helper of the GPU tests against torch's own e4m3."""
 import ctypes as C
+import os
+import re
+import subprocess
 
 import pytest
 import torch
@@ -8,6 +11,9 @@ import torch
 from hashattention import _ops
 from tests import fp8_util as ref
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "hashattention-1.0_amd", "csrc")
+HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 NULL, SHAPE, DTYPE, ALIGN, WS, NODEV = -1, -2, -3, -4, -5, -6
 BF16, F32, E4M3 = _ops.HA_BF16, _ops.HA_F32, _ops.HA_FP8_E4M3
 
@@ -116,3 +122,29 @@ def test_the_64_bit_helper_rounds_as_torch_does():
     y = torch.randn(3, 300, dtype=torch.float64)
     q, s = ref.quantise(y)
     assert torch.allclose(_ops.fp8_values(q, s, 300).double(), y, rtol=2.0 ** -4 * 1.01, atol=float(s.max()) * 2.0 ** -10)
+
+
+@pytest.mark.skipif(not os.path.exists(HIPCC), reason="hipcc not available")
+def test_what_the_counted_waits_rely_on():
+    """The staged kernels count their own requests: in the loops around their matrix instructions there is no other vector memory
+    access (a spilled register would be one), and nothing but the requests writes M0."""
+    from importlib import util
+    spec = util.spec_from_file_location("hashattn_build", os.path.join(ROOT, "hashattention-1.0_amd", "build.py"))
+    mod = util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    flags = [f for f in mod.FLAGS if f != "-shared"]
+    r = subprocess.run([HIPCC, *flags, "-S", "--cuda-device-only", "-I", os.path.join(ROOT, "include"), "-I", CSRC,
+                        os.path.join(CSRC, "ha_linear_fp8.hip"), "-o", "-"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+    scratch = dict(re.findall(r"\.name:\s+(\S+)\n\s+\.private_segment_fixed_size: (\d+)", r.stdout))
+    assert scratch and not {n: b for n, b in scratch.items() if b != "0"}
+    staged = [n for n in scratch if "tiled_kernel" in n]
+    assert len(staged) >= 6
+    for name in staged:
+        body = r.stdout[r.stdout.index("\n" + name + ":"):]
+        lines = body[:body.index("s_endpgm")].splitlines()
+        mfma = [i for i, line in enumerate(lines) if "v_mfma" in line]
+        inside = [line.strip() for line in lines[mfma[0]:mfma[-1]]]
+        foreign = [line for line in inside if re.match(r"(global_|flat_|scratch_|buffer_)", line) and not line.endswith(" lds")]
+        assert not foreign, (name, foreign[:3])
+        assert not [line for line in lines if re.search(r"\bm0\b", line) and not line.strip().startswith(("s_mov_b32 m0,", ";"))], name

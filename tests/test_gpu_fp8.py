@@ -440,6 +440,25 @@ def test_in_a_graph_and_on_another_stream(m):
         assert torch.equal(on_side, bufs[0][-1])
 
 
+@pytest.mark.parametrize("m,n,k,glu", [(300, 2000, 2200, False), (2100, 6200, 1000, False), (2100, 6200, 4096, True), (700, 300, 4000, True),
+                                       (4096, 4096, 128, False), (2048, 8192, 300, False)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_counted_waits_and_full_waits_give_the_same_bits(m, n, k, glu, out_dtype):
+    """The staged kernels wait for counted requests; the library's twin waits for all of them."""
+    q, s, wq, ws = make_linear(m, n, k, seed=31, glu=glu)
+    w = _ops.pack_weight_fp8(wq, scales=ws, glu=glu)
+    main, twin = _ops.load_library(), _ops.load_wait_all_variant()
+    outs = []
+    for lib in (main, twin, main):
+        _ops._lib = lib
+        try:
+            outs.append(_ops.linear_fp8(q, s, w, torch.empty(m, n // 2 if glu else n, dtype=out_dtype, device=DEV), swiglu=glu))
+            torch.cuda.synchronize()
+        finally:
+            _ops._lib = main
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
 def test_refusals_of_the_bindings():
     x = torch.zeros(4, 256, dtype=torch.bfloat16, device=DEV)
     q, s = _ops.fp8_rows(4, 256, DEV)
