@@ -118,6 +118,18 @@ def test_swiglu_far_gates():
     assert v[2, :128].isnan().all() and v[2, 128:].isfinite().all()
 
 
+@pytest.mark.parametrize("gate", [88.0, -86.0, 1e4, 2.0e38, 2.4e38, 3.4e38])
+def test_swiglu_gates_up_to_the_largest_number(gate):
+    """silu(g) = g up to the largest fp32 number, whose product with log2(e) overflows."""
+    x = torch.zeros(2, 2 * 128, device=DEV)
+    x[:, :128] = gate
+    x[:, 128:] = torch.linspace(0.5, 1.0, 128, device=DEV) * (1e-35 if gate > 1e30 else 1.0)
+    q, s = rows(2, 128)
+    _ops.swiglu_fp8(x, q, s)
+    g, u = x[:, :128].double(), x[:, 128:].double()
+    ref.assert_rows(q, s, g * torch.sigmoid(g) * u, 2.0 ** -20)
+
+
 # ------------------------------------------------------------------------------------------ norm
 
 # sum of squares: at most 64 additions in a thread, 6 + 16 across them, each 2^-24 of a positive total; the root halves that;
