@@ -930,6 +930,11 @@ def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: to
     q_sm, s_sm = _fp8_rows_of(q, scales, m, k)
     if glu != swiglu:
         raise ValueError("swiglu takes weights packed with glu, and nothing else does")
+    count = (((n >> 1) + 7) // 8 if glu else (n + 15) // 16) * ((k + 127) // 128)
+    if tiles.dtype != torch.uint8 or tile_scales.dtype != torch.float32 or tiles.numel() != 2048 * count or tile_scales.numel() != 2 * count \
+            or not (tiles.is_contiguous() and tile_scales.is_contiguous()):
+        raise ValueError(f"weight must be as pack_weight_fp8 leaves it for [{n}, {k}]: uint8 tiles and fp32 scales, got {tiles.dtype} "
+                         f"{tuple(tiles.shape)} and {tile_scales.dtype} {tuple(tile_scales.shape)}")
     o_sm = _rows_of(out, "out", m, n // 2 if swiglu else n)
     r, r_sm = None, 0
     if residual is not None:
@@ -942,6 +947,8 @@ def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: to
         ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
     elif ws is not None:
         _same_device(out, ws)
+        if not ws.is_contiguous():
+            raise ValueError("ws must be contiguous")
     _launch_on(dev, lib.ha_linear_fp8, "ha_linear_fp8",
                (q.data_ptr(), q_sm, scales.data_ptr(), s_sm, tiles.data_ptr(), tile_scales.data_ptr(), r, r_sm, 1 if swiglu else 0,
                 out.data_ptr(), o_sm, _DTYPE[out.dtype], m, n, k, None if ws is None else ws.data_ptr(),

@@ -24,7 +24,7 @@ __all__ = ["Fp8Linear", "convert_fp8", "stacked_weight"]
 
 class Fp8Linear(nn.Module):
     """`nn.Linear` for inference with its weight in 8 bits.  `tiles` and `tile_scales` are buffers (`_ops.pack_weight_fp8`), so the
-    module moves and is saved like any other."""
+    module moves and is saved like any other.  Casts of the model to another type leave both as they are."""
 
     def __init__(self, weight: _ops.Fp8Weight, bias: Optional[torch.Tensor] = None):
         super().__init__()
@@ -43,7 +43,17 @@ class Fp8Linear(nn.Module):
     def packed(self) -> _ops.Fp8Weight:
         return _ops.Fp8Weight(self.tiles, self.tile_scales, self.out_features, self.in_features, False)
 
+    def _apply(self, fn, recurse=True):
+        # casts (`model.bfloat16()`, `model.to(dtype)`) skip integers: the scales pass as their bits and stay fp32
+        self.tile_scales = self.tile_scales.view(torch.int32)
+        try:
+            return super()._apply(fn, recurse)
+        finally:
+            self.tile_scales = self.tile_scales.view(torch.float32)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1:] != (self.in_features,):
+            raise ValueError(f"x has rows of {tuple(x.shape[-1:])}, the weight takes {self.in_features}")
         if torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("Fp8Linear is for inference: no gradient flows through the 8-bit product (use torch.no_grad())")
         rows = x.reshape(-1, self.in_features)
@@ -68,14 +78,15 @@ def _stacks(modules: Sequence[Fp8Linear]) -> bool:
 
 def stacked_weight(owner: nn.Module, name: str, modules: Sequence[Fp8Linear]) -> _ops.Fp8Weight:
     """The modules' weights as one matrix, rows behind each other, kept on `owner` under `name`.  Packed tiles are ordered by row, so
-    the modules' own buffers become parts of the stacked ones: nothing is held twice.  Rebuilt when a module's buffer was
-    replaced (a move to another device, a loaded state dict)."""
-    key = tuple(t.data_ptr() for m in modules for t in (m.tiles, m.tile_scales))
-    hit = owner.__dict__.get(name)
-    if hit is not None and hit[0] == key:
-        return hit[1]
+    the modules' own buffers become parts of the stacked ones: nothing is held twice.  Rebuilt when a module's buffer is no longer
+    that part (a move to another device, a loaded state dict): call it once before a graph is captured."""
+    weight = owner.__dict__.get(name)
+    if weight is not None and _parts_of(weight, modules):
+        return weight
     if not _stacks(modules):
         raise ValueError("rows of packed weights stack in whole tiles of 16")
+    if modules[0].tiles.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the projections' weights are not stacked yet: run one step before capturing a graph")
     tiles, scales = torch.cat([m.tiles for m in modules]), torch.cat([m.tile_scales for m in modules])
     at = s_at = 0
     for m in modules:
@@ -83,8 +94,19 @@ def stacked_weight(owner: nn.Module, name: str, modules: Sequence[Fp8Linear]) ->
         m.tiles, m.tile_scales = tiles[at:at + n], scales[s_at:s_at + ns]
         at, s_at = at + n, s_at + ns
     weight = _ops.Fp8Weight(tiles, scales, sum(m.out_features for m in modules), modules[0].in_features, False)
-    owner.__dict__[name] = (tuple(t.data_ptr() for m in modules for t in (m.tiles, m.tile_scales)), weight)
+    owner.__dict__[name] = weight
     return weight
+
+
+def _parts_of(weight: _ops.Fp8Weight, modules: Sequence[Fp8Linear]) -> bool:
+    """Whether the modules' buffers are the stacked weight's memory, in order (it is alive, so no other tensor can lie there)."""
+    at, s_at = weight.tiles.data_ptr(), weight.scales.data_ptr()
+    for m in modules:
+        tiles, scales = m.tiles, m.tile_scales
+        if tiles.data_ptr() != at or scales.data_ptr() != s_at:
+            return False
+        at, s_at = at + tiles.numel(), s_at + 4 * scales.numel()
+    return True
 
 
 _ATTENTION, _MLP = ("q_proj", "k_proj", "v_proj", "o_proj"), ("gate_proj", "up_proj", "down_proj")

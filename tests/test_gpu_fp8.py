@@ -501,6 +501,14 @@ def test_refusals_of_the_bindings():
         lambda: _ops.linear_fp8(q, s, w, out.double()),
         lambda: _ops.linear_fp8(q, s, w, out, residual=out.bfloat16()),
         lambda: _ops.linear_fp8(q[:, :128], s[:, :1], w, out),
+        # weights that are not as they were packed
+        lambda: _ops.linear_fp8(q, s, w._replace(scales=w.scales.bfloat16()), out),
+        lambda: _ops.linear_fp8(q, s, w._replace(scales=w.scales[1:]), out),
+        lambda: _ops.linear_fp8(q, s, w._replace(tiles=w.tiles[:2048]), out),
+        lambda: _ops.linear_fp8(q, s, w._replace(tiles=w.tiles.float()), out),
+        lambda: _ops.linear_fp8(q, s, w._replace(N=64), torch.empty(4, 64, device=DEV)),
+        lambda: _ops.linear_fp8(q, s, w._replace(tiles=w.tiles.expand(2, -1)[:, ::2]), out),
+        lambda: _ops.linear_fp8(q, s, w, out, ws=torch.empty(64, dtype=torch.uint8, device=DEV)[::2]),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(ValueError):

@@ -191,3 +191,67 @@ def test_decoder_with_8_bit_projections_generates_from_one_graph(dtype):
     dec.fill_cache_synthetic(100)
     with torch.no_grad():
         assert torch.isfinite(dec.decode_step(torch.arange(5, device=DEV))).all()
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.float(), lambda m: m.to(torch.bfloat16), lambda m: m.cpu().to(DEV).half()])
+def test_casting_a_model_keeps_the_packed_weights(cast):
+    """The scales stay fp32, and the same rows give the same product."""
+    torch.manual_seed(4)
+    model = nn.Sequential(nn.Linear(300, 200), nn.Linear(200, 40)).to(DEV)
+    model[0] = fp8.Fp8Linear.from_linear(model[0])
+    tiles, scales = model[0].tiles.clone(), model[0].tile_scales.clone()
+    x = torch.randn(3, 300, device=DEV).half().float()
+    with torch.no_grad():
+        want = model[0](x) - model[0].bias
+        cast(model)
+        assert model[0].tile_scales.dtype == torch.float32 and torch.equal(model[0].tile_scales, scales) and torch.equal(model[0].tiles, tiles)
+        assert model[0].bias.dtype == model[1].weight.dtype
+        model[0].bias.zero_()
+        want2 = model[0](x)
+    assert torch.allclose(want2, want, rtol=0, atol=2.0 ** -20 * float(want.abs().max() + 1))     # the bias came off with two roundings
+
+
+def test_stacked_weights_follow_copies_and_replacements():
+    """A deep copy of a model has its own stacked weight; buffers put in place of others are taken up, also where memory is reused."""
+    import copy
+    torch.manual_seed(5)
+    parts = nn.ModuleList([fp8.Fp8Linear.from_linear(nn.Linear(256, n, bias=False).to(DEV)) for n in (64, 32)])
+    q, s = _ops.fp8_rows(3, 256, DEV)
+    _ops.quantize_rows_fp8(torch.randn(3, 256, device=DEV), q, s)
+
+    def product(owner):
+        return _ops.linear_fp8(q, s, fp8.stacked_weight(owner, "_stack", list(owner)), torch.empty(3, 96, device=DEV))
+
+    def single(owner):
+        return torch.cat([_ops.linear_fp8(q, s, m.packed, torch.empty(3, m.out_features, device=DEV)) for m in owner], dim=1)
+
+    assert torch.equal(product(parts), single(parts))
+    twin = copy.deepcopy(parts)
+    with torch.no_grad():
+        parts[0].tiles.zero_()
+    assert torch.equal(product(parts), single(parts)) and torch.equal(product(twin), single(twin))
+    assert not torch.equal(product(parts), product(twin))
+    del parts
+    new = fp8.Fp8Linear.from_linear(nn.Linear(256, 64, bias=False).to(DEV))
+    twin[0].load_state_dict(new.state_dict(), assign=True)
+    assert torch.equal(product(twin), single(twin))
+    assert torch.equal(product(twin)[:, :64], _ops.linear_fp8(q, s, new.packed, torch.empty(3, 64, device=DEV)))
+
+
+def test_stacking_inside_a_capture_is_refused():
+    parts = [fp8.Fp8Linear.from_linear(nn.Linear(128, 16, bias=False).to(DEV)) for _ in range(2)]
+    owner, x = nn.Module(), torch.zeros(4, device=DEV)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="before capturing"):
+            fp8.stacked_weight(owner, "_stack", parts)
+    w = fp8.stacked_weight(owner, "_stack", parts)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        x.add_(1)
+        assert fp8.stacked_weight(owner, "_stack", parts) is w
+
+
+def test_rows_of_another_width_are_refused():
+    mod = fp8.Fp8Linear.from_linear(nn.Linear(128, 16).to(DEV))
+    with pytest.raises(ValueError):
+        mod(torch.zeros(4, 64, device=DEV))
