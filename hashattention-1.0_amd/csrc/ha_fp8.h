@@ -14,6 +14,11 @@
 #define HA_FP8_MAX 448.0f
 #define HA_FP8_FLOOR 0x1p-96f
 
+#define HA_FP8_MAX_K (2147483647 - HA_FP8_BLOCK)  // a row's positions, rounded up to whole blocks, are 32-bit
+
+// a launch holds fewer than 2^32 threads
+static inline bool ha_fits_launch(int64_t groups, int threads) { return groups <= 0xFFFFFFFFLL / threads; }
+
 static inline int ha_fp8_blocks(int K) { return K / HA_FP8_BLOCK + (K % HA_FP8_BLOCK != 0); }
 
 #ifdef __HIPCC__

@@ -140,11 +140,11 @@ __global__ __launch_bounds__(T) void rmsnorm_fp8_kernel(const char *x, int64_t x
 
 int check_rows(const void *q, int64_t q_stride_m, const float *scales, int64_t s_stride_m, int M, int K) {
     HA_REQUIRE(M == 0 || (q && scales), HA_ERR_NULL_POINTER, "q/scales is NULL");
-    HA_REQUIRE(M >= 0 && K >= 1, HA_ERR_BAD_SHAPE, "need M >= 0 rows of K >= 1 elements");
+    HA_REQUIRE(M >= 0 && K >= 1 && K <= HA_FP8_MAX_K, HA_ERR_BAD_SHAPE, "need M >= 0 rows of K >= 1 elements, K <= %d", HA_FP8_MAX_K);
     const int64_t kb = ha_fp8_blocks(K);
     HA_REQUIRE(q_stride_m >= kb * HA_FP8_BLOCK && s_stride_m >= kb, HA_ERR_BAD_SHAPE,
                "a row of q spans ha_fp8_row_bytes(K) bytes and a row of scales one number per block of 128");
-    HA_REQUIRE((int64_t)M * kb <= 2147483647LL, HA_ERR_BAD_SHAPE, "too many blocks for one launch");
+    HA_REQUIRE(ha_fits_launch((M * kb + 15) / 16, 256), HA_ERR_BAD_SHAPE, "too many blocks for one launch");
     HA_REQUIRE(ha_aligned(q, 16) && q_stride_m % 16 == 0 && ha_aligned(scales, 4), HA_ERR_MISALIGNED, "rows of q must be 16-byte aligned");
     return HA_OK;
 }
@@ -217,6 +217,7 @@ int ha_rmsnorm_fp8(const void *x, int64_t x_stride_m, const void *residual, int6
     int st = check_rows(q, q_stride_m, scales, scales_stride_m, M, K);
     if (st) return st;
     HA_REQUIRE(K <= 65536, HA_ERR_BAD_SHAPE, "rows of up to 65536 elements");
+    HA_REQUIRE(ha_fits_launch(M, K <= 512 ? 64 : K <= 8192 ? 256 : 1024), HA_ERR_BAD_SHAPE, "too many rows for one launch");
     HA_REQUIRE(x_stride_m >= K && (!residual || residual_stride_m >= K) && (!sum_out || sum_stride_m >= K) && eps >= 0.f, HA_ERR_BAD_SHAPE,
                "strides smaller than a row, or a negative eps");
     const int es = ha_dtype_bytes(dtype);

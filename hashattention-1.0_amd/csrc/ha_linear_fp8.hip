@@ -865,12 +865,12 @@ int ha_pack_weight_fp8(const void *w, int64_t w_stride_n, int dtype, const float
     HA_REQUIRE(dtype == HA_F32 || dtype == HA_BF16 || dtype == HA_F16 || dtype == HA_FP8_E4M3, HA_ERR_BAD_DTYPE, "unknown dtype %d", dtype);
     HA_REQUIRE((dtype == HA_FP8_E4M3) == (w_scales != nullptr), HA_ERR_NULL_POINTER,
                "weights in e4m3 come with their scales, any other type without");
-    HA_REQUIRE(N >= 1 && K >= 1 && w_stride_n >= K && (glu == 0 || (glu == 1 && N % 2 == 0)), HA_ERR_BAD_SHAPE,
-               "need N, K >= 1, an even N for the gate/up form, rows of at least K elements");
+    HA_REQUIRE(N >= 1 && K >= 1 && K <= HA_FP8_MAX_K && w_stride_n >= K && (glu == 0 || (glu == 1 && N % 2 == 0)), HA_ERR_BAD_SHAPE,
+               "need N >= 1, 1 <= K <= %d, an even N for the gate/up form, rows of at least K elements", HA_FP8_MAX_K);
     const Packed p = packed_shape(N, K, glu);
     const int rows = glu ? N / 2 : N, row_blocks = ha_fp8_blocks(rows);
     HA_REQUIRE(!w_scales || w_scales_stride_n >= p.kb, HA_ERR_BAD_SHAPE, "a row of w_scales holds a number for every block of 128 inputs");
-    HA_REQUIRE(row_blocks * (glu ? 2LL : 1LL) <= 65535, HA_ERR_BAD_SHAPE, "matrix too large for one launch");
+    HA_REQUIRE(row_blocks * (glu ? 2LL : 1LL) <= 65535 && ha_fits_launch(p.kb, 256), HA_ERR_BAD_SHAPE, "matrix too large for one launch");
     HA_REQUIRE(ha_aligned(w, dtype == HA_FP8_E4M3 ? 1 : ha_dtype_bytes(dtype)) && ha_aligned(w_scales, 4) && ha_aligned(tiles, 16) &&
                    ha_aligned(tile_scales, 8),
                HA_ERR_MISALIGNED, "tiles must be 16-byte aligned, the others to their elements");
@@ -888,7 +888,7 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
     HA_REQUIRE(tiles && tile_scales && (M == 0 || (xq && x_scales && out)), HA_ERR_NULL_POINTER,
                "xq/x_scales/tiles/tile_scales/out is NULL");
     HA_REQUIRE(out_dtype == HA_F32 || out_dtype == HA_BF16 || out_dtype == HA_F16, HA_ERR_BAD_DTYPE, "unknown dtype %d", out_dtype);
-    HA_REQUIRE(M >= 0 && N >= 1 && K >= 1, HA_ERR_BAD_SHAPE, "need M >= 0, N >= 1, K >= 1");
+    HA_REQUIRE(M >= 0 && N >= 1 && K >= 1 && K <= HA_FP8_MAX_K, HA_ERR_BAD_SHAPE, "need M >= 0, N >= 1, 1 <= K <= %d", HA_FP8_MAX_K);
     HA_REQUIRE(act == HA_ACT_NONE || act == HA_ACT_SWIGLU, HA_ERR_BAD_SHAPE, "unknown activation %d", act);
     HA_REQUIRE(!act || (N % 2 == 0 && !residual), HA_ERR_BAD_SHAPE, "SwiGLU needs an even number of weight rows and no residual");
     const Packed p = packed_shape(N, K, act);
@@ -907,9 +907,12 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
     const Args a = {(hipStream_t)stream, (const uint8_t *)xq, xq_stride_m, x_scales, x_scales_stride_m, (const uint8_t *)tiles, tile_scales, ep,
                     M, N, act, p};
     const bool exact = out_dtype == HA_F32;
-    HA_REQUIRE(((int64_t)M + 15) / 16 * (p.n_tiles + 7LL) <= 2147483647LL, HA_ERR_BAD_SHAPE, "too many tiles for one launch");
     // offsets within a workgroup's tiles are 32-bit
-    const bool in_reach = 256 * (xq_stride_m + x_scales_stride_m * 4) < (1LL << 31) && (int64_t)p.kb * kTileBytes * 16 < (1LL << 31);
+    const bool in_reach = xq_stride_m < (1LL << 22) && x_scales_stride_m < (1LL << 20) && (int64_t)p.kb * kTileBytes * 16 < (1LL << 31);
+    const int64_t groups = M <= 16               ? p.n_tiles + 7LL
+                           : in_reach && M > 128 ? ((M + 127LL) / 128) * ((p.n_tiles + 7LL) / 8) + 7
+                                                 : ((M + 31LL) / 32) * ((p.n_tiles + 1LL) / 2 + 7);
+    HA_REQUIRE(ha_fits_launch(groups, M <= 16 ? 1024 : in_reach && M > 128 ? 256 : 512), HA_ERR_BAD_SHAPE, "too many tiles for one launch");
     const Splits splits = in_reach ? splits_for(M, p) : Splits{1, p.kb};
     if (splits.count > 1) {
         const size_t need = ha_linear_fp8_workspace_bytes(M, N, K, act);

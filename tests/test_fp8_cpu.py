@@ -61,6 +61,13 @@ def test_row_operators_refuse(lib, mem):
         assert f(M=-1) == SHAPE and f(K=0) == SHAPE and f(xs=255) == SHAPE and f(qs=255) == SHAPE and f(ss=1) == SHAPE
         assert f(K=2 ** 31 - 1, xs=2 ** 33, qs=2 ** 31, ss=2 ** 24, M=2 ** 10) == SHAPE            # more blocks than a launch takes
         assert f(q=mem + 8) == ALIGN and f(qs=264) == ALIGN and f(s=mem + 2) == ALIGN and f(x=mem + 1) == ALIGN
+        # a launch holds fewer than 2^32 threads: 2^28 - 16 blocks of 128, 2^26 - 1 narrow rows to normalise
+        assert f(K=128, qs=128, ss=1, M=2 ** 28 + 1) == SHAPE and f(K=2 ** 31 - 1, xs=2 ** 33, qs=2 ** 31, ss=2 ** 24, M=1) == SHAPE
+    if lib.ha_device_count() == 0:
+        assert rows(K=128, qs=128, ss=1, M=2 ** 28 - 16) == NODEV and glu(K=128, qs=128, ss=1, M=2 ** 28 - 16) == NODEV
+        assert norm(K=128, qs=128, ss=1, M=2 ** 26 - 1) == NODEV
+        assert rows(K=2 ** 31 - 129, xs=2 ** 33, qs=2 ** 31, ss=2 ** 24, M=1) == NODEV
+    assert norm(K=128, qs=128, ss=1, M=2 ** 26) == SHAPE and norm(K=4096, xs=4096, qs=4096, ss=32, M=2 ** 24) == SHAPE
     assert norm(w=None) == NULL and norm(r=mem, rs=255) == SHAPE and norm(h=mem, hs=255) == SHAPE and norm(eps=-1.0) == SHAPE
     assert norm(K=65537, xs=65537, qs=65664, ss=513) == SHAPE
     assert norm(w=mem + 1) == ALIGN and norm(r=mem + 1, rs=256) == ALIGN and norm(h=mem + 1, hs=256) == ALIGN
@@ -90,6 +97,13 @@ def test_pack_and_linear_refuse(lib, mem):
     assert lin(x=mem + 8) == ALIGN and lin(xs=264) == ALIGN and lin(t=mem + 8) == ALIGN and lin(ts=mem + 4) == ALIGN
     assert lin(s=mem + 2) == ALIGN and lin(o=mem + 1) == ALIGN and lin(r=mem + 1, rs=32) == ALIGN
     assert lin(M=2 ** 31 - 1, N=2 ** 31 - 1, os=2 ** 31) == SHAPE
+    # positions in a row and threads in a launch are 32-bit
+    huge = dict(K=2 ** 31 - 1, xs=2 ** 31, ss=2 ** 24)
+    assert lin(**huge) == SHAPE and pack(K=2 ** 31 - 1, sn=2 ** 31) == SHAPE
+    assert lin(N=2 ** 27, os=2 ** 27) == SHAPE and lin(M=300, xs=2 ** 62, ss=2 ** 62, N=2 ** 31 - 1, os=2 ** 31) == SHAPE
+    if lib.ha_device_count() == 0:
+        assert lin(N=2 ** 25, os=2 ** 25) == NODEV and lin(M=2 ** 19, N=2 ** 18, os=2 ** 18) == NODEV
+        assert lin(M=300, xs=2 ** 62, ss=2 ** 62) == NODEV                  # strides whose products leave 64 bits
     # sizes whose sums go through a workspace: missing, too small, misaligned
     big = dict(M=300, N=32, K=4096, xs=4096, ss=32)
     need = lib.ha_linear_fp8_workspace_bytes(300, 32, 4096, 0)
