@@ -12,35 +12,66 @@ namespace {
 template <typename E>
 constexpr int dtype_of = __is_same(E, ElemF32) ? HA_F32 : __is_same(E, ElemBF16) ? HA_BF16 : HA_F16;
 
-// eight consecutive elements row[k0 .. k0 + 8) of a row of K, zero beyond K.  VEC: rows are 16-byte aligned.
-template <typename E, bool VEC>
-__device__ __forceinline__ void load8_guarded(const char *row, int k0, int K, float (&f)[8]) {
-    if (VEC && k0 + 8 <= K) {
-        Elem<E>::unpack(Elem<E>::load8(row, k0 / 8), f);
-        return;
-    }
+// Rows begin anywhere (an odd width moves every row off the last one's alignment): 16 bytes at the address of an element are one
+// load all the same, which the hardware takes at any alignment.
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_anywhere __attribute__((aligned(2)));
+template <typename E>
+struct Eight {
+    u32x4 v[Elem<E>::bytes / 2];
+};
+
+// eight consecutive elements row[k0 .. k0 + 8) of a row of K, zero beyond K
+template <typename E>
+__device__ __forceinline__ Eight<E> load8(const char *row, int k0, int K) {
+    constexpr int es = Elem<E>::bytes;
+    Eight<E> r;
+    if (k0 + 8 <= K) {
+        const u32x4_anywhere *p = reinterpret_cast<const u32x4_anywhere *>(row + (int64_t)k0 * es);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = k0 + i < K ? ha_load_elem(row, k0 + i, dtype_of<E>) : 0.f;
+        for (int i = 0; i < es / 2; ++i) r.v[i] = p[i];
+        return r;
+    }
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = k0 + i >= K ? 0u : es == 4 ? ((const uint32_t *)row)[k0 + i] : (uint32_t)((const uint16_t *)row)[k0 + i];
+    if constexpr (es == 4) {
+        r.v[0] = u32x4{w[0], w[1], w[2], w[3]};
+        r.v[1] = u32x4{w[4], w[5], w[6], w[7]};
+    } else {
+        r.v[0] = u32x4{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
+    }
+    return r;
+}
+template <typename E>
+__device__ __forceinline__ void to_float(const Eight<E> &r, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (Elem<E>::bytes == 4)
+            f[i] = __uint_as_float(r.v[i >> 2][i & 3]);
+        else if constexpr (__is_same(E, ElemBF16))
+            f[i] = __uint_as_float(i & 1 ? r.v[0][i >> 1] & 0xFFFF0000u : r.v[0][i >> 1] << 16);
+        else
+            f[i] = __half2float(__ushort_as_half((unsigned short)(r.v[0][i >> 1] >> (16 * (i & 1)))));
+    }
 }
 
 // eight elements that are already rounded to E, stored at row[k0 .. min(k0 + 8, K))
-template <typename E, bool VEC>
-__device__ __forceinline__ void store8_guarded(char *row, int k0, int K, const float (&f)[8]) {
-    if (VEC && k0 + 8 <= K) {
-        if constexpr (Elem<E>::bytes == 4) {
-            float4 *p = reinterpret_cast<float4 *>(row + (int64_t)k0 * 4);
-            p[0] = make_float4(f[0], f[1], f[2], f[3]);
-            p[1] = make_float4(f[4], f[5], f[6], f[7]);
-        } else {
-            uint32_t w[4];
+template <typename E>
+__device__ __forceinline__ void store8(char *row, int k0, int K, const float (&f)[8]) {
+    if (k0 + 8 <= K) {
+        u32x4_anywhere *p = reinterpret_cast<u32x4_anywhere *>(row + (int64_t)k0 * Elem<E>::bytes);
+        uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (__is_same(E, ElemBF16))
-                    w[i] = (__float_as_uint(f[2 * i]) >> 16) | (__float_as_uint(f[2 * i + 1]) & 0xFFFF0000u);
-                else
-                    w[i] = (uint32_t)__half_as_ushort(__float2half(f[2 * i])) | ((uint32_t)__half_as_ushort(__float2half(f[2 * i + 1])) << 16);
-            }
-            *reinterpret_cast<uint4 *>(row + (int64_t)k0 * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (__is_same(E, ElemF16)) w[i] = (uint32_t)__half_as_ushort(__float2half(f[i]));
+            else w[i] = __float_as_uint(f[i]) >> (__is_same(E, ElemBF16) ? 16 : 0);
+        }
+        if constexpr (Elem<E>::bytes == 4) {
+            p[0] = u32x4{w[0], w[1], w[2], w[3]};
+            p[1] = u32x4{w[4], w[5], w[6], w[7]};
+        } else {
+            p[0] = u32x4{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
         }
         return;
     }
@@ -64,7 +95,7 @@ __device__ __forceinline__ void write_block(const float (&y)[8], int sub, uint8_
 
 // One block of 128 per 16 lanes, eight elements per lane; blocks of all rows in one flat order, so that narrow rows fill a
 // workgroup too.  PAIR: x holds [gate | up] rows of 2 K elements and the block is that of silu(gate) * up.
-template <typename E, bool VEC, bool PAIR>
+template <typename E, bool PAIR>
 __global__ __launch_bounds__(256) void rows_fp8_kernel(const char *__restrict__ x, int64_t x_sb, int n_blocks, int kb_count, int K,
                                                        uint8_t *__restrict__ q, int64_t q_sm, float *__restrict__ scales, int64_t s_sm) {
     const int sub = threadIdx.x & 15;
@@ -73,10 +104,10 @@ __global__ __launch_bounds__(256) void rows_fp8_kernel(const char *__restrict__ 
     const int m = blk / kb_count, kb = blk - m * kb_count, k0 = kb * HA_FP8_BLOCK + sub * 8;
     const char *row = x + m * x_sb;
     float y[8];
-    load8_guarded<E, VEC>(row, k0, K, y);
+    to_float<E>(load8<E>(row, k0, K), y);
     if constexpr (PAIR) {
         float u[8];
-        load8_guarded<E, VEC>(row + (int64_t)K * Elem<E>::bytes, k0, K, u);
+        to_float<E>(load8<E>(row + (int64_t)K * Elem<E>::bytes, k0, K), u);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = ha_silu(y[i]) * u[i];
     }
@@ -86,7 +117,7 @@ __global__ __launch_bounds__(256) void rows_fp8_kernel(const char *__restrict__ 
 // One workgroup of T threads per row, the row in registers between the sum of squares and the scaling (PER x 8 elements per
 // thread).  h = x + residual is rounded to the element type first: what is stored for the next addition is what is normalised.
 // h may be stored over x or the residual: every thread has read its elements of both before it stores them.
-template <typename E, bool VEC, int T, int PER>
+template <typename E, int T, int PER>
 __global__ __launch_bounds__(T) void rmsnorm_fp8_kernel(const char *x, int64_t x_sb, const char *res, int64_t res_sb,
                                                         const char *__restrict__ w, int K, float eps, char *sum_out, int64_t sum_sb,
                                                         uint8_t *__restrict__ q, int64_t q_sm, float *__restrict__ scales, int64_t s_sm) {
@@ -94,20 +125,27 @@ __global__ __launch_bounds__(T) void rmsnorm_fp8_kernel(const char *x, int64_t x
     const int tid = threadIdx.x;
     const int64_t m = blockIdx.x;
     float h[PER][8], a = 0.f;
+    // the weights are requested with the row, ahead of the sum that the scaling waits for, where registers allow it
+    constexpr bool kAhead = PER <= 4;
+    Eight<E> ahead[kAhead ? PER : 1];
+    if constexpr (kAhead) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) load8_guarded<E, VEC>(x + m * x_sb, (tid + i * T) * 8, K, h[i]);
+        for (int i = 0; i < PER; ++i) ahead[i] = load8<E>(w, (tid + i * T) * 8, K);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) to_float<E>(load8<E>(x + m * x_sb, (tid + i * T) * 8, K), h[i]);
     if (res) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             float r[8];
-            load8_guarded<E, VEC>(res + m * res_sb, (tid + i * T) * 8, K, r);
+            to_float<E>(load8<E>(res + m * res_sb, (tid + i * T) * 8, K), r);
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[i][j] = ha_round_to(h[i][j] + r[j], dtype_of<E>);
         }
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        if (sum_out) store8_guarded<E, VEC>(sum_out + m * sum_sb, (tid + i * T) * 8, K, h[i]);
+        if (sum_out) store8<E>(sum_out + m * sum_sb, (tid + i * T) * 8, K, h[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) a = fmaf(h[i][j], h[i][j], a);
     }
@@ -126,7 +164,8 @@ __global__ __launch_bounds__(T) void rmsnorm_fp8_kernel(const char *x, int64_t x
         const int k0 = (tid + i * T) * 8;
         if (k0 / HA_FP8_BLOCK * HA_FP8_BLOCK >= K) continue;  // whole groups of 16 lanes: the block lies beyond the row
         float g[8];
-        load8_guarded<E, VEC>(w, k0, K, g);
+        if constexpr (kAhead) to_float<E>(ahead[i], g);
+        else to_float<E>(load8<E>(w, k0, K), g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] = h[i][j] * rstd * g[j];
         if (k0 + 8 > K) {  // 0 * infinity at the padding would be NaN
@@ -149,28 +188,21 @@ int check_rows(const void *q, int64_t q_stride_m, const float *scales, int64_t s
     return HA_OK;
 }
 
-// 16-byte loads of rows `stride` elements apart
-bool rows_aligned(const void *p, int64_t stride, int dtype) { return ha_aligned(p, 16) && stride * ha_dtype_bytes(dtype) % 16 == 0; }
-
 template <bool PAIR>
 int launch_rows(const void *x, int64_t x_stride_m, int dtype, int M, int K, void *q, int64_t q_stride_m, float *scales, int64_t s_stride_m,
                 void *stream) {
     const int kb = ha_fp8_blocks(K), n = M * kb;
     const unsigned grid = (unsigned)((n + 15LL) / 16);
-    const bool vec = rows_aligned(x, x_stride_m, dtype) && (!PAIR || (int64_t)K * ha_dtype_bytes(dtype) % 16 == 0);
     const int64_t x_sb = x_stride_m * ha_dtype_bytes(dtype);
-#define HA_ROWS(E_, V_)                                                                                                                 \
-    hipLaunchKernelGGL((rows_fp8_kernel<E_, V_, PAIR>), dim3(grid), dim3(256), 0, (hipStream_t)stream, (const char *)x, x_sb, n, kb, K, \
+#define HA_ROWS(E_)                                                                                                                 \
+    hipLaunchKernelGGL((rows_fp8_kernel<E_, PAIR>), dim3(grid), dim3(256), 0, (hipStream_t)stream, (const char *)x, x_sb, n, kb, K, \
                        (uint8_t *)q, q_stride_m, scales, s_stride_m)
     if (dtype == HA_F32) {
-        if (vec) HA_ROWS(ElemF32, true);
-        else HA_ROWS(ElemF32, false);
+        HA_ROWS(ElemF32);
     } else if (dtype == HA_BF16) {
-        if (vec) HA_ROWS(ElemBF16, true);
-        else HA_ROWS(ElemBF16, false);
+        HA_ROWS(ElemBF16);
     } else {
-        if (vec) HA_ROWS(ElemF16, true);
-        else HA_ROWS(ElemF16, false);
+        HA_ROWS(ElemF16);
     }
 #undef HA_ROWS
     HA_CHECK_LAUNCH("rows_fp8_kernel");
@@ -225,30 +257,25 @@ int ha_rmsnorm_fp8(const void *x, int64_t x_stride_m, const void *residual, int6
                "pointers are not aligned to their elements");
     st = ha_require_device();
     if (st || M == 0) return st;
-    const bool vec = rows_aligned(x, x_stride_m, dtype) && ha_aligned(weight, 16) && (!residual || rows_aligned(residual, residual_stride_m, dtype)) &&
-                     (!sum_out || rows_aligned(sum_out, sum_stride_m, dtype));
-#define HA_NORM(E_, V_, T_, P_)                                                                                                          \
-    hipLaunchKernelGGL((rmsnorm_fp8_kernel<E_, V_, T_, P_>), dim3((unsigned)M), dim3(T_), 0, (hipStream_t)stream, (const char *)x,       \
+#define HA_NORM(E_, T_, P_)                                                                                                          \
+    hipLaunchKernelGGL((rmsnorm_fp8_kernel<E_, T_, P_>), dim3((unsigned)M), dim3(T_), 0, (hipStream_t)stream, (const char *)x,       \
                        x_stride_m * es, (const char *)residual, residual_stride_m * es, (const char *)weight, K, eps, (char *)sum_out,    \
                        sum_stride_m * es, (uint8_t *)q, q_stride_m, scales, scales_stride_m)
-#define HA_NORM_SIZE(E_, V_)                            \
+#define HA_NORM_SIZE(E_)                            \
     do {                                                \
-        if (K <= 512) HA_NORM(E_, V_, 64, 1);           \
-        else if (K <= 2048) HA_NORM(E_, V_, 256, 1);    \
-        else if (K <= 4096) HA_NORM(E_, V_, 256, 2);    \
-        else if (K <= 8192) HA_NORM(E_, V_, 256, 4);    \
-        else if (K <= 16384) HA_NORM(E_, V_, 1024, 2);  \
-        else HA_NORM(E_, V_, 1024, 8);                  \
+        if (K <= 512) HA_NORM(E_, 64, 1);           \
+        else if (K <= 2048) HA_NORM(E_, 256, 1);    \
+        else if (K <= 4096) HA_NORM(E_, 256, 2);    \
+        else if (K <= 8192) HA_NORM(E_, 256, 4);    \
+        else if (K <= 16384) HA_NORM(E_, 1024, 2);  \
+        else HA_NORM(E_, 1024, 8);                  \
     } while (0)
     if (dtype == HA_F32) {
-        if (vec) HA_NORM_SIZE(ElemF32, true);
-        else HA_NORM_SIZE(ElemF32, false);
+        HA_NORM_SIZE(ElemF32);
     } else if (dtype == HA_BF16) {
-        if (vec) HA_NORM_SIZE(ElemBF16, true);
-        else HA_NORM_SIZE(ElemBF16, false);
+        HA_NORM_SIZE(ElemBF16);
     } else {
-        if (vec) HA_NORM_SIZE(ElemF16, true);
-        else HA_NORM_SIZE(ElemF16, false);
+        HA_NORM_SIZE(ElemF16);
     }
 #undef HA_NORM_SIZE
 #undef HA_NORM

@@ -516,7 +516,7 @@ int ha_linear_tiled(const void *x, int64_t x_stride_m, const void *tiles, const 
  *                          8 bits.  sum_out (may be NULL): h [M, K], which the layer's next addition takes; it may be x's or the
  *                          residual's own memory (same pointer and stride), any other overlap is not supported.  K <= 65536
  *   ha_swiglu_fp8          gate_up [M, 2 F] (gate | up): silu(gate) * up in fp32 and straight to 8 bits, rows of F
- * Any alignment of x, weight, residual and sum_out to their elements is taken; rows on 16-byte boundaries are read faster.
+ * Rows of x, residual and sum_out and the weight may begin at any element.
  *
  * Weights are packed once, in the order the matrix instruction reads them:
  *   ha_weight_fp8_bytes / _scales   sizes of the packed copy of a [N, K] matrix: bytes of `tiles`, floats of `tile_scales` (0 for
