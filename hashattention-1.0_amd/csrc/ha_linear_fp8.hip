@@ -225,8 +225,8 @@ __device__ __forceinline__ void join_waves(const float (&s_c)[NWAVE][16 * NT][16
 // ---- any size: NT tiles of 16 weight rows and 16 MT rows of x per workgroup, straight from memory to registers
 //
 // The waves cut K into slices and walk them in groups of PF blocks, weights and rows of x requested together, a group ahead, without
-// a barrier; their sums are joined through LDS.  Eight waves with a block or two each on its way keep more bytes in flight than
-// staging through LDS would, which is what a matrix of few tiles needs; NT and MT set how often x and the weights are read from L2.
+// a barrier; their sums are joined through LDS.  For rows too long for registers: up to 16 rows, 17 to 32 where the tiles need no cut
+// of K, and rows of x so far apart that a group's positions pass 32 bits.  NT and MT set how often x and the weights are read.
 template <int NWAVE, int PF, int NT, int MT, bool EXACT, bool GLU>
 __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_stream_kernel(const uint8_t *__restrict__ x, int64_t x_sm, const float *__restrict__ xs,
                                                                        int64_t xs_sm, const uint8_t *__restrict__ tiles,
@@ -338,7 +338,8 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_rows_kernel(const uint8
                                                                      const float *__restrict__ ws, Epilogue ep, int M, int N, int kb_count,
                                                                      int n_tiles, int groups_m) {
     static_assert(KW % PF == 0, "a slice is whole groups of blocks");
-    __shared__ float s_c[NWAVE][16][16 * MT + 1];
+    __shared__ float s_c[2][NWAVE][16][16 * MT + 1];
+    __shared__ u32x4 s_x[NWAVE][128];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, g = lane >> 4;
     // workgroups go to the XCDs in turn: the groups of rows that walk the same tiles share an XCD and its L2
     const int turn = (int)(blockIdx.x >> 3), step = (int)(gridDim.x / (unsigned)groups_m);
@@ -365,20 +366,58 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_rows_kernel(const uint8
     if (nt >= n_tiles) return;
     Group now, next;
     fetch(now, nt, 0);  // the first weights are on their way before x is set up
+    // Rows of x are read as whole lines of 128 bytes, eight to a load, and turned through LDS into the operand's order (row r: chunks g
+    // and 4 + g), two KiB per wave; chunk c of row r lies in place c ^ (r & 7) of its line, which keeps both sides free of bank
+    // conflicts.  Read in the operand's order, 16 rows at a time, a load takes half lines of twice as many, and x is what a
+    // workgroup waits for first.  A row's scales are consecutive: one load for the slice, moved where the slice ends behind K.
+    // (6144 x 4096, 128 rows: 19.3 us with x in the operand's order and scales one by one, 16.0 with the scales' load, 13.2 with both.)
     u32x4 xa[KW][MT], xb[KW][MT];
     float xsc[KW][MT];
 #pragma unroll
     for (int j = 0; j < KW; ++j)
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const int64_t m = min(m0 + 16 * t + r, M - 1);
-            const int kb = min(kb0 + j, kb_count - 1);
-            const u32x4 *xp = reinterpret_cast<const u32x4 *>(x + m * x_sm + kb * HA_FP8_BLOCK + g * 16);
-            xa[j][t] = xp[0];
-            xb[j][t] = xp[4];
-            xsc[j][t] = xs[m * xs_sm + kb];
+            const uint8_t *xp = x + min(kb0 + j, kb_count - 1) * HA_FP8_BLOCK + (lane & 7) * 16;
+            xa[j][t] = *reinterpret_cast<const u32x4 *>(xp + (int64_t)min(m0 + 16 * t + (lane >> 3), M - 1) * x_sm);
+            xb[j][t] = *reinterpret_cast<const u32x4 *>(xp + (int64_t)min(m0 + 16 * t + 8 + (lane >> 3), M - 1) * x_sm);
+        }
+    const int s_from = max(min(kb0, kb_count - KW), 0), s_past = kb0 - s_from;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const float *sp = xs + (int64_t)min(m0 + 16 * t + r, M - 1) * xs_sm + s_from;
+        float v[KW];
+        if constexpr (KW == 1) {
+            v[0] = sp[0];
+        } else {
+            typedef float run __attribute__((ext_vector_type(KW), aligned(4)));
+            const run f = *reinterpret_cast<const run *>(sp);
+#pragma unroll
+            for (int j = 0; j < KW; ++j) v[j] = f[j];
+        }
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+            xsc[j][t] = v[j];
+#pragma unroll
+            for (int d = 1; j + d < KW; ++d)
+                if (s_past == d) xsc[j][t] = v[j + d];
+        }
+    }
+    u32x4 *turn_x = s_x[wave];
+#pragma unroll
+    for (int j = 0; j < KW; ++j)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            turn_x[(lane >> 3) * 8 + ((lane & 7) ^ (lane >> 3))] = xa[j][t];
+            turn_x[(8 + (lane >> 3)) * 8 + ((lane & 7) ^ (lane >> 3))] = xb[j][t];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's LDS accesses stay in this order
+            __builtin_amdgcn_wave_barrier();
+            xa[j][t] = turn_x[r * 8 + (g ^ (r & 7))];
+            xb[j][t] = turn_x[r * 8 + ((4 + g) ^ (r & 7))];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
     f32x4 acc[MT];
+    int side = 0;
     auto multiply = [&](const Group &w, int j0) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
@@ -417,10 +456,10 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_rows_kernel(const uint8
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s_c[wave][4 * g + i][16 * t + r] = acc[t][i];
+            for (int i = 0; i < 4; ++i) s_c[side][wave][4 * g + i][16 * t + r] = acc[t][i];
         __syncthreads();
-        join_waves<NWAVE, 1, MT, GLU>(s_c, ep, nt, m0, M, N);
-        if (more) __syncthreads();  // the sums are read: the next tile's may overwrite them
+        join_waves<NWAVE, 1, MT, GLU>(s_c[side], ep, nt, m0, M, N);
+        side ^= 1;  // the next tile's sums go to the other buffer; a wave is back at this one only behind the barrier in between
     };
     for (; nt + step < n_tiles; nt += step) tile(nt, nt + step, true);
     tile(nt, nt, false);
@@ -754,7 +793,8 @@ struct Args {
 template <int NWAVE, int KW, int PF, int MT, bool WIDE, bool EXACT>
 void launch_rows(const Args &a) {
     const int groups = (a.M + 16 * MT - 1) / (16 * MT);
-    const int rounds = (int)(((int64_t)a.p.n_tiles * groups + 255) / 256);
+    // every CU a workgroup (two of those that would fit bring nothing), an eighth of them to each XCD; the tiles in equal rounds
+    const int most = groups <= 32 ? 256 / groups / 8 * 8 : 8, rounds = (a.p.n_tiles + most - 1) / most;
     const unsigned grid = (unsigned)groups * (unsigned)(((a.p.n_tiles + rounds - 1) / rounds + 7) / 8 * 8);
     if (a.act)
         hipLaunchKernelGGL((linear_fp8_rows_kernel<NWAVE, KW, PF, MT, WIDE, EXACT, true>), dim3(grid), dim3(NWAVE * 64), 0, a.stream, a.x,
@@ -790,14 +830,11 @@ void launch_tiled(const Args &a) {
                            a.p.kb, nullptr);
 }
 
-// Whether x of 17 to 128 rows stays in registers, weights streamed past it: rows of 16 to 32 blocks.  Against tiles with K cut
-// (6144 x 4096): 32 rows 11.4 us (13.7), 64 rows 17.4 (15.7), 128 rows 19.3 (19.7); of few tiles (1024 x 4096) only up to 32 rows: 9.1
-// us (10.2), 64 rows 14.6 (11.0).
-bool keeps_rows(int M, Packed p) { return M <= 128 && p.kb >= 16 && p.kb <= 32 && (M <= 32 || p.n_tiles > 128); }
-
-// Whether a product of short rows is too small for tiles: 64 rows of x and 32 of weights per workgroup straight from memory, while
-// that is two workgroups per CU at most (2048 x 512: 256 rows 5.3 us against 9.2, 512 rows 8.7 against 9.4, 1024 rows 11.8 against 9.6).
-bool short_rows(int M, Packed p) { return p.kb <= 16 && ((M + 63LL) / 64) * ((p.n_tiles + 1LL) / 2) <= 512; }
+// Whether x of 17 rows and more stays in registers, weights streamed past it: rows of up to 32 blocks, and at most six tiles for a
+// workgroup (N / 16 tiles times M / 64 groups of rows, over 256 workgroups).  Against tiles of 128 x 128, with K cut where
+// they are few: 6144 x 4096, 64 rows 11.3 us (15.9), 128 rows 13.2 (19.7), 256 rows 18.7 (23.9); 4096 x 2304, 256 rows 13.4 (18.9),
+// 384 rows, six tiles, 19.4 (17.9); 6144 x 2048, 384 rows, nine tiles, 25.7 (18.8).  128 rows and fewer would not fill a tile.
+bool keeps_rows(int M, Packed p) { return p.kb <= 32 && (M <= 128 || ((M + 63LL) / 64) * p.n_tiles <= 1536); }
 
 // How many ways K is cut for tiles of 128 x 128: into as many as give every CU a tile, of at least four blocks (cut for two
 // tiles per CU instead, the longer sum of the parts costs more than it brings: 4096 x 14336, 256 rows 41 us against 37; not cut 96).
@@ -805,7 +842,7 @@ struct Splits {
     int count, per;
 };
 Splits splits_for(int M, Packed p) {
-    if (M <= 16 || p.kb < 8 || keeps_rows(M, p) || short_rows(M, p)) return {1, p.kb};
+    if (M <= 16 || keeps_rows(M, p)) return {1, p.kb};
     const int64_t tiles = ((p.n_tiles + 7LL) / 8) * ((M + 127LL) / 128);
     int64_t want = 256 / tiles;
     if (want > p.kb / 4) want = p.kb / 4;
@@ -828,15 +865,17 @@ void launch_split(const Args &a, Splits s, float *partial) {
         hipLaunchKernelGGL(join_splits_kernel<false>, dim3(grid), dim3(256), 0, a.stream, partial, s.count, a.ep, a.M, a.N, a.p.n_tiles);
 }
 
-// 17 rows and more without tiles
+// 17 rows and more, in registers
 template <bool EXACT>
 void launch_some_rows(const Args &a) {
-    if (keeps_rows(a.M, a.p)) {
-        if (a.M <= 32) launch_rows<8, 4, 4, 2, false, EXACT>(a);
-        else launch_rows<8, 4, 2, 4, false, EXACT>(a);
+    if (a.M <= 32) {
+        if (a.p.kb <= 8) launch_rows<8, 1, 1, 2, false, EXACT>(a);
+        else if (a.p.kb <= 16) launch_rows<8, 2, 2, 2, false, EXACT>(a);
+        else launch_rows<8, 4, 4, 2, false, EXACT>(a);
     } else {
-        if (a.M <= 32) launch_stream<8, 2, 2, 2, EXACT>(a);
-        else launch_stream<8, 1, 2, 4, EXACT>(a);
+        if (a.p.kb <= 8) launch_rows<8, 1, 1, 4, false, EXACT>(a);
+        else if (a.p.kb <= 16) launch_rows<8, 2, 2, 4, false, EXACT>(a);
+        else launch_rows<8, 4, 2, 4, false, EXACT>(a);
     }
 }
 
@@ -909,10 +948,11 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
     const bool exact = out_dtype == HA_F32;
     // offsets within a workgroup's tiles are 32-bit
     const bool in_reach = xq_stride_m < (1LL << 22) && x_scales_stride_m < (1LL << 20) && (int64_t)p.kb * kTileBytes * 16 < (1LL << 31);
-    const int64_t groups = M <= 16               ? p.n_tiles + 7LL
-                           : in_reach && M > 128 ? ((M + 127LL) / 128) * ((p.n_tiles + 7LL) / 8) + 7
-                                                 : ((M + 31LL) / 32) * ((p.n_tiles + 1LL) / 2 + 7);
-    HA_REQUIRE(ha_fits_launch(groups, M <= 16 ? 1024 : in_reach && M > 128 ? 256 : 512), HA_ERR_BAD_SHAPE, "too many tiles for one launch");
+    const bool tiled = in_reach && M > 32;
+    const int64_t groups = M <= 16 ? p.n_tiles + 7LL
+                           : tiled ? ((M + 127LL) / 128) * ((p.n_tiles + 7LL) / 8) + 7
+                                   : ((M + 31LL) / 32) * ((p.n_tiles + 1LL) / 2 + 7);
+    HA_REQUIRE(ha_fits_launch(groups, M <= 16 ? 1024 : tiled ? 256 : 512), HA_ERR_BAD_SHAPE, "too many tiles for one launch");
     const Splits splits = in_reach ? splits_for(M, p) : Splits{1, p.kb};
     if (splits.count > 1) {
         const size_t need = ha_linear_fp8_workspace_bytes(M, N, K, act);
@@ -924,20 +964,23 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
     if (splits.count > 1) {
         if (exact) launch_split<true>(a, splits, (float *)workspace);
         else launch_split<false>(a, splits, (float *)workspace);
-    } else if (in_reach && M > 128 && !short_rows(M, p)) {
-        const int64_t big = ((p.n_tiles + 15LL) / 16) * ((M + 255LL) / 256);
-        if (exact) launch_tiled<2, 2, 4, 4, 1, true>(a);
-        else if (big >= 200) launch_tiled<2, 4, 8, 4, 3, false>(a);
-        else launch_tiled<2, 2, 4, 4, 1, false>(a);
     } else if (M <= 16) {
         if (p.kb <= 8) launch_rows<8, 1, 1, 1, true, true>(a);
         else if (p.kb <= 16) launch_rows<8, 2, 2, 1, true, true>(a);
         else if (p.kb <= 32) launch_rows<8, 4, 2, 1, true, true>(a);
         else launch_stream<16, 2, 1, 1, true>(a);
-    } else if (exact) {
-        launch_some_rows<true>(a);
+    } else if (keeps_rows(M, p)) {
+        if (exact) launch_some_rows<true>(a);
+        else launch_some_rows<false>(a);
+    } else if (tiled) {
+        // (up to 32 rows the stream is as fast; 17408 x 4224, 40 rows 29.8 us against the stream's 34.1, 128 rows 36.5 against 66)
+        const int64_t big = ((p.n_tiles + 15LL) / 16) * ((M + 255LL) / 256);
+        if (exact) launch_tiled<2, 2, 4, 4, 1, true>(a);
+        else if (big >= 200) launch_tiled<2, 4, 8, 4, 3, false>(a);
+        else launch_tiled<2, 2, 4, 4, 1, false>(a);
     } else {
-        launch_some_rows<false>(a);
+        if (exact) launch_stream<8, 2, 2, 2, true>(a);
+        else launch_stream<8, 2, 2, 2, false>(a);
     }
     HA_CHECK_LAUNCH("ha_linear_fp8");
     return HA_OK;

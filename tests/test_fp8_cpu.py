@@ -105,13 +105,13 @@ def test_pack_and_linear_refuse(lib, mem):
         assert lin(N=2 ** 25, os=2 ** 25) == NODEV and lin(M=2 ** 19, N=2 ** 18, os=2 ** 18) == NODEV
         assert lin(M=300, xs=2 ** 62, ss=2 ** 62) == NODEV                  # strides whose products leave 64 bits
     # sizes whose sums go through a workspace: missing, too small, misaligned
-    big = dict(M=300, N=32, K=4096, xs=4096, ss=32)
-    need = lib.ha_linear_fp8_workspace_bytes(300, 32, 4096, 0)
-    assert need == 8 * 300 * 32 * 4
+    big = dict(M=300, N=32, K=8192, xs=8192, ss=64)
+    need = lib.ha_linear_fp8_workspace_bytes(300, 32, 8192, 0)
+    assert need == 16 * 300 * 32 * 4
     assert lin(**big) == WS and lin(**big, ws=mem, wsb=need - 1) == WS and lin(**big, ws=mem + 8, wsb=need) == ALIGN
-    for m, n, k, act in ((4, 32, 4096, 0), (16, 4096, 14336, 0), (64, 6144, 4096, 0), (4096, 28672, 4096, 0), (0, 32, 4096, 0), (300, 33, 4096, 1)):
+    for m, n, k, act in ((4, 32, 4096, 0), (16, 4096, 14336, 0), (64, 6144, 4096, 0), (4096, 28672, 4096, 0), (0, 32, 8192, 0), (300, 33, 8192, 1), (300, 32, 4096, 0)):
         assert lib.ha_linear_fp8_workspace_bytes(m, n, k, act) == 0
-    assert lib.ha_linear_fp8_workspace_bytes(300, 33, 4096, 0) > 0
+    assert lib.ha_linear_fp8_workspace_bytes(300, 33, 8192, 0) > 0
     assert _ops.LINEAR_FP8_UNSPLIT_ROWS == 16 and lib.ha_linear_fp8_workspace_bytes(17, 32, 14336, 0) > 0
     if lib.ha_device_count() == 0:
         assert pack() == NODEV and lin() == NODEV and lin(**big, ws=mem, wsb=need) == NODEV

@@ -220,7 +220,11 @@ LINEAR_SIZES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (4, 6144, 4096), (4, 4096
                 (31, 48, 1000), (33, 1000, 127), (64, 512, 4096), (65, 257, 640), (100, 1000, 1111), (128, 512, 1024), (200, 640, 384),
                 (256, 256, 2048), (300, 129, 2000), (513, 384, 512), (1000, 1030, 900), (2048, 1024, 512),
                 (20, 130, 4200), (40, 300, 14336), (90, 1000, 2200), (130, 2000, 4000), (257, 700, 1100), (700, 3000, 640),
-                (3000, 5000, 300)]
+                (3000, 5000, 300),
+                # rows in registers over several groups of rows and rounds of tiles, on both sides of every length they are cut at
+                (24, 6200, 1000), (48, 9000, 1024), (130, 4200, 1025), (192, 6144, 2048), (200, 5000, 2049), (500, 1700, 4096), (17, 8200, 4000),
+                # K cut, and whole tiles of both sizes
+                (17, 64, 4097), (300, 515, 8192), (1000, 300, 5000), (900, 2000, 4200), (28, 17000, 4200), (50, 17000, 4200), (1030, 1600, 700), (4200, 3300, 257)]
 
 
 @pytest.mark.parametrize("out_dtype", DTYPES)
@@ -236,7 +240,7 @@ def test_linear(m, n, k, out_dtype):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 33, 100), (4, 4096, 1024), (20, 200, 300), (48, 300, 1111), (130, 384, 640), (512, 512, 256), (700, 1000, 384),
-                                   (50, 260, 4300), (300, 515, 1200), (2100, 6000, 200)])
+                                   (50, 260, 4300), (300, 515, 1200), (2100, 6000, 200), (300, 515, 4900), (700, 2700, 300)])
 @pytest.mark.parametrize("out_dtype", DTYPES)
 def test_linear_residual(m, n, k, out_dtype):
     q, s, wq, ws = make_linear(m, n, k, seed=1)
@@ -251,7 +255,8 @@ def test_linear_residual(m, n, k, out_dtype):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 2, 128), (4, 28672, 512), (16, 2 * 37, 300), (17, 2 * 130, 257), (40, 2 * 200, 1000), (129, 2 * 256, 384),
-                                   (520, 2 * 384, 256), (600, 2 * 333, 500), (60, 2 * 1001, 4096), (150, 2 * 515, 1500), (2100, 2 * 3001, 200)])
+                                   (520, 2 * 384, 256), (600, 2 * 333, 500), (60, 2 * 1001, 4096), (150, 2 * 515, 1500), (2100, 2 * 3001, 200),
+                                   (150, 2 * 515, 4900), (700, 2 * 1351, 300), (200, 2 * 3100, 2500)])
 @pytest.mark.parametrize("out_dtype", DTYPES)
 def test_linear_swiglu(m, n, k, out_dtype):
     q, s, wq, ws = make_linear(m, n, k, seed=3, glu=True)
@@ -261,27 +266,38 @@ def test_linear_swiglu(m, n, k, out_dtype):
     ref.assert_linear(out, *ref.linear(q, s, wq, ws, k, glu=True, eight_bit_sums=eight_bit_sums(m, out_dtype)))
 
 
-@pytest.mark.parametrize("m", [3, 40, 300])
-def test_linear_strides(m):
+@pytest.mark.parametrize("m,n,k", [(3, 200, 300), (40, 200, 300), (300, 200, 300), (700, 2600, 300), (2100, 6000, 300), (300, 200, 4300), (5, 200, 4300)])
+def test_linear_strides(m, n, k):
     """Rows of x, scales, residual and out that are parts of wider ones; what lies beside them stays."""
-    n, k = 200, 300
+    kb = ref.blocks(k)
     q, s, wq, ws = make_linear(m, n, k, seed=4)
     w = _ops.pack_weight_fp8(wq, scales=ws)
-    wide_q = torch.full((m, 512), 0x7f, dtype=torch.uint8, device=DEV)          # NaN beside the rows
-    wide_q[:, 64:64 + 384] = q.view(torch.uint8)
-    wide_s = torch.full((m, 7), float("nan"), device=DEV)
-    wide_s[:, 2:5] = s
+    wide_q = torch.full((m, 128 * (kb + 1)), 0x7f, dtype=torch.uint8, device=DEV)          # NaN beside the rows
+    wide_q[:, 64:64 + 128 * kb] = q.view(torch.uint8)
+    wide_s = torch.full((m, kb + 4), float("nan"), device=DEV)
+    wide_s[:, 2:2 + kb] = s
     wide_r = torch.full((m, n + 3), float("nan"), dtype=torch.bfloat16, device=DEV)
     wide_r[:, 1:n + 1] = noise(m, n, seed=5).bfloat16()
     wide_o = torch.full((m + 1, n + 5), 9.0, dtype=torch.bfloat16, device=DEV)
-    _ops.linear_fp8(wide_q[:, 64:64 + 384].view(torch.float8_e4m3fn), wide_s[:, 2:5], w, wide_o[:m, 3:n + 3], residual=wide_r[:, 1:n + 1])
+    _ops.linear_fp8(wide_q[:, 64:64 + 128 * kb].view(torch.float8_e4m3fn), wide_s[:, 2:2 + kb], w, wide_o[:m, 3:n + 3], residual=wide_r[:, 1:n + 1])
     ref.assert_linear(wide_o[:m, 3:n + 3], *ref.linear(q, s, wq, ws, k, residual=wide_r[:, 1:n + 1], eight_bit_sums=eight_bit_sums(m, torch.bfloat16)))
     assert (wide_o[:, :3] == 9.0).all() and (wide_o[:, n + 3:] == 9.0).all() and (wide_o[m] == 9.0).all()
 
 
-@pytest.mark.parametrize("m", [5, 30, 64, 300, 600])
-def test_linear_rows_keep_their_nan_to_themselves(m):
-    n, k = 384, 512
+@pytest.mark.parametrize("m,n,k", [(3, 100, 300), (40, 100, 300), (40, 300, 4300), (150, 300, 4300)])
+def test_linear_rows_far_apart(m, n, k):
+    """Rows of x four MiB and more apart: positions within a group of rows pass 32 bits."""
+    q, s, wq, ws = make_linear(m, n, k, seed=14)
+    w = _ops.pack_weight_fp8(wq, scales=ws)
+    far = torch.empty(m, (1 << 24) // (2 if m > 100 else 1), dtype=torch.uint8, device=DEV)[:, 32:32 + q.shape[1]]
+    far.copy_(q.view(torch.uint8))
+    out = _ops.linear_fp8(far.view(torch.float8_e4m3fn), s, w, torch.empty(m, n, dtype=torch.bfloat16, device=DEV))
+    ref.assert_linear(out, *ref.linear(q, s, wq, ws, k, eight_bit_sums=eight_bit_sums(m, torch.bfloat16)))
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 384, 512), (30, 384, 512), (64, 384, 512), (300, 384, 512), (600, 384, 512), (1100, 1500, 512), (64, 384, 4224),
+                                   (6, 384, 4224), (100, 384, 4096)])
+def test_linear_rows_keep_their_nan_to_themselves(m, n, k):
     q, s, wq, ws = make_linear(m, n, k, seed=6)
     w = _ops.pack_weight_fp8(wq, scales=ws)
     clean = _ops.linear_fp8(q, s, w, torch.empty(m, n, device=DEV))
@@ -350,7 +366,7 @@ def test_packing_takes_numbers_and_scales_over_as_they_are():
     ref.assert_linear(out, *ref.linear(q, s, wq, ws, k))
 
 
-@pytest.mark.parametrize("m,n,k", [(40, 300, 4300), (300, 512, 2304)])
+@pytest.mark.parametrize("m,n,k", [(40, 300, 4300), (300, 512, 8192)])
 def test_linear_with_a_workspace_of_the_callers(m, n, k):
     """The same bits from the caller's scratch as from the allocator's; what lies behind the bytes asked for stays; too little is refused."""
     q, s, wq, ws = make_linear(m, n, k, seed=21)
@@ -453,7 +469,7 @@ def test_in_a_graph_and_on_another_stream(m):
 
 
 @pytest.mark.parametrize("m,n,k,glu", [(300, 2000, 2200, False), (2100, 6200, 1000, False), (2100, 6200, 4096, True), (700, 300, 4000, True),
-                                       (4096, 4096, 128, False), (2048, 8192, 300, False)])
+                                       (4096, 4096, 128, False), (2048, 8192, 300, False), (700, 300, 5000, True), (1000, 3000, 2200, False)])
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
 def test_counted_waits_and_full_waits_give_the_same_bits(m, n, k, glu, out_dtype):
     """The staged kernels wait for counted requests; the library's twin waits for all of them."""
