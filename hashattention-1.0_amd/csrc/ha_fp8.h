@@ -35,12 +35,18 @@ __device__ __forceinline__ uint32_t ha_abs_bits(float y) { return __float_as_uin
 struct HaFp8Scale {
     float scale, inv;
 };
-__device__ __forceinline__ HaFp8Scale ha_fp8_scale(uint32_t top_bits) {
-    const float a = __uint_as_float(top_bits);
-    const float f = a < HA_FP8_FLOOR ? HA_FP8_FLOOR : a;  // a NaN compares false and stays
+// The numbers of the block are y = p * common; top_bits is the largest |p|.  inv turns a p (not a y) into its e4m3 number: a factor
+// that all share falls out of p / |p|max, and its rounding with it.
+__device__ __forceinline__ HaFp8Scale ha_fp8_scale(uint32_t top_bits, float common = 1.0f) {
+    const float a = __uint_as_float(top_bits), f = a * common;
     HaFp8Scale r;
-    r.inv = HA_FP8_MAX / f;
-    r.scale = top_bits == 0u ? 1.0f : f / HA_FP8_MAX;
+    if (f < HA_FP8_FLOOR) {  // a NaN compares false
+        r.inv = HA_FP8_MAX / HA_FP8_FLOOR * common;
+        r.scale = top_bits == 0u ? 1.0f : HA_FP8_FLOOR / HA_FP8_MAX;
+    } else {
+        r.inv = HA_FP8_MAX / a;
+        r.scale = f / HA_FP8_MAX;
+    }
     return r;
 }
 

@@ -80,14 +80,15 @@ __device__ __forceinline__ void store8(char *row, int k0, int K, const float (&f
         if (k0 + i < K) Elem<E>::store1(row, k0 + i, f[i]);
 }
 
-// The 16 lanes that share a block find its largest magnitude, then each writes its eight e4m3 bytes and the first the scale.
-__device__ __forceinline__ void write_block(const float (&y)[8], int sub, uint8_t *q8, float *scale) {
+// The 16 lanes that share a block (of numbers y * common) find its largest magnitude, then each writes its eight e4m3 bytes and
+// the first the scale.
+__device__ __forceinline__ void write_block(const float (&y)[8], float common, int sub, uint8_t *q8, float *scale) {
     uint32_t top = 0u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, ha_abs_bits(y[i]));
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 16));
-    const HaFp8Scale s = ha_fp8_scale(top);
+    const HaFp8Scale s = ha_fp8_scale(top, common);
     *reinterpret_cast<uint2 *>(q8) = make_uint2(ha_fp8x4(y[0] * s.inv, y[1] * s.inv, y[2] * s.inv, y[3] * s.inv),
                                                 ha_fp8x4(y[4] * s.inv, y[5] * s.inv, y[6] * s.inv, y[7] * s.inv));
     if (sub == 0) *scale = s.scale;
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(256) void rows_fp8_kernel(const char *__restrict__ 
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = ha_silu(y[i]) * u[i];
     }
-    write_block(y, sub, q + m * q_sm + k0, scales + m * s_sm + kb);
+    write_block(y, 1.0f, sub, q + m * q_sm + k0, scales + m * s_sm + kb);
 }
 
 // One workgroup of T threads per row, the row in registers between the sum of squares and the scaling (PER x 8 elements per
@@ -159,6 +160,11 @@ __global__ __launch_bounds__(T) void rmsnorm_fp8_kernel(const char *x, int64_t x
         for (int i = 0; i < T / 64; ++i) a += s_sum[i];
     }
     const float rstd = 1.0f / sqrtf(a / (float)K + eps);
+    // Its power of two scales the row exactly; what is left, 1 to 2, is common to every block and only the block's scale takes it.
+    // So the numbers carry the product's rounding alone, none in 16 bits, and neither the root's nor its reciprocal's, and as few
+    // of them as can be land on the other side of an e4m3 step.  A NaN's power is infinity: the row is NaN.
+    const float power = __uint_as_float(__float_as_uint(rstd) & 0x7F800000u);
+    const float common = __uint_as_float((__float_as_uint(rstd) & 0x007FFFFFu) | 0x3F800000u);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int k0 = (tid + i * T) * 8;
@@ -167,13 +173,13 @@ __global__ __launch_bounds__(T) void rmsnorm_fp8_kernel(const char *x, int64_t x
         if constexpr (kAhead) to_float<E>(ahead[i], g);
         else to_float<E>(load8<E>(w, k0, K), g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = h[i][j] * rstd * g[j];
+        for (int j = 0; j < 8; ++j) g[j] = h[i][j] * power * g[j];
         if (k0 + 8 > K) {  // 0 * infinity at the padding would be NaN
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (k0 + j >= K) g[j] = 0.f;
         }
-        write_block(g, tid & 15, q + m * q_sm + k0, scales + m * s_sm + k0 / HA_FP8_BLOCK);
+        write_block(g, common, tid & 15, q + m * q_sm + k0, scales + m * s_sm + k0 / HA_FP8_BLOCK);
     }
 }
 
