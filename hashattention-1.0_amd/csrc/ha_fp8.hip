@@ -95,7 +95,8 @@ __device__ __forceinline__ void write_block(const float (&y)[8], float common, i
 }
 
 // One block of 128 per 16 lanes, eight elements per lane; blocks of all rows in one flat order, so that narrow rows fill a
-// workgroup too.  PAIR: x holds [gate | up] rows of 2 K elements and the block is that of silu(gate) * up.
+// workgroup too.  PAIR: x holds [gate | up] rows of 2 K elements and the block is that of silu(gate) * up.  Bound by memory: SwiGLU of
+// 4096 x 14336 58 us (60.6 at a large copy's rate), rows of 8192 x 4096 21 us; 4 x 4096 2.1 us, a launch's length.
 template <typename E, bool PAIR>
 __global__ __launch_bounds__(256) void rows_fp8_kernel(const char *__restrict__ x, int64_t x_sb, int n_blocks, int kb_count, int K,
                                                        uint8_t *__restrict__ q, int64_t q_sm, float *__restrict__ scales, int64_t s_sm) {
@@ -117,7 +118,8 @@ __global__ __launch_bounds__(256) void rows_fp8_kernel(const char *__restrict__ 
 
 // One workgroup of T threads per row, the row in registers between the sum of squares and the scaling (PER x 8 elements per
 // thread).  h = x + residual is rounded to the element type first: what is stored for the next addition is what is normalised.
-// h may be stored over x or the residual: every thread has read its elements of both before it stores them.
+// h may be stored over x or the residual: every thread has read its elements of both before it stores them.  Bound by memory: 8192 x
+// 4096 with a residual 46 us (48.4 at a large copy's rate); 4 x 4096 3.9 us, one row's chain of load, sum, barrier and write.
 template <typename E, int T, int PER>
 __global__ __launch_bounds__(T) void rmsnorm_fp8_kernel(const char *x, int64_t x_sb, const char *res, int64_t res_sb,
                                                         const char *__restrict__ w, int K, float eps, char *sum_out, int64_t sum_sb,

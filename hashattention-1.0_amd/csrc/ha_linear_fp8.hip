@@ -227,6 +227,8 @@ __device__ __forceinline__ void join_waves(const float (&s_c)[NWAVE][16 * NT][16
 // The waves cut K into slices and walk them in groups of PF blocks, weights and rows of x requested together, a group ahead, without
 // a barrier; their sums are joined through LDS.  For rows too long for registers: up to 16 rows, 17 to 32 where the tiles need no cut
 // of K, and rows of x so far apart that a group's positions pass 32 bits.  NT and MT set how often x and the weights are read.
+// Bound by the stream of weights: 4 rows, 4096 x 14336, 11.8 us (5.0 TB/s; 9.7 at the rate of a plain read); 16 rows 15.9 us, the
+// rows of x beside it.
 template <int NWAVE, int PF, int NT, int MT, bool EXACT, bool GLU>
 __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_stream_kernel(const uint8_t *__restrict__ x, int64_t x_sm, const float *__restrict__ xs,
                                                                        int64_t xs_sm, const uint8_t *__restrict__ tiles,
@@ -330,8 +332,10 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_stream_kernel(const uin
 //
 // The waves of a workgroup cut K into slices of KW blocks; each keeps its slice of 16 MT rows of x in registers (as e4m3, 8
 // registers per block and 16 rows; widened when used) and walks the weight tiles blockIdx, blockIdx + step, ...: per tile KW
-// blocks of 2 KiB, consecutive in memory, requested a whole tile ahead.  The waves' sums are joined through LDS.  What bounds it is
-// the stream of weights; the conversions (16 per block and 16 rows) and the matrix instructions run under it.
+// blocks of 2 KiB, consecutive in memory, requested PF blocks ahead.  The waves' sums are joined through LDS.  What bounds it is
+// the stream of weights (16 rows, 28672 x 4096 with SwiGLU, 20.4 us, 5.8 TB/s); the conversions (16 per block and 16 rows) and the
+// matrix instructions run under it.  With more rows it is the start, x out of L2 into every workgroup, and about 2.6 us per tile
+// behind it (6144 x 4096, three tiles: 128 rows 13.2 us).
 template <int NWAVE, int KW, int PF, int MT, bool WIDE, bool EXACT, bool GLU>
 __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_rows_kernel(const uint8_t *__restrict__ x, int64_t x_sm, const float *__restrict__ xs,
                                                                      int64_t xs_sm, const uint8_t *__restrict__ tiles,
@@ -468,7 +472,8 @@ __global__ __launch_bounds__(NWAVE * 64) void linear_fp8_rows_kernel(const uint8
 // ---- many rows: tiles of BN weight rows x BM rows of x per workgroup, staged through LDS
 //
 // WN x WM waves of TN x TM operand tiles each (16 weight rows, 16 rows of x).  Everything a block of 128 inputs needs travels
-// from memory straight to LDS (one KiB per request and wave).  Weights lie there in the order the matrix instruction takes
+// from memory straight to LDS (one KiB per request and wave).  Bound by the matrix cores with the blocks' scales (a multiply-add per
+// result and block) beside them: 4096 x 28672 x 4096 in 480 - 500 us, 2.0 PFLOP/s.  Weights lie there in the order the matrix instruction takes
 // them, lane l's 16 bytes at l * 16.  Rows of x arrive as whole 128-byte lines, eight to a request; the 16-byte chunk c of row r
 // sits in place c ^ (r & 7) of its line - each lane asks for the chunk that belongs in its place - so that the eight lanes that an
 // LDS read serves at a time, same chunk of eight rows, meet eight different bank groups.
@@ -788,12 +793,11 @@ struct Args {
     Packed p;
 };
 
-// One workgroup per CU (two of them, with x not widened to make room: 28672 x 4096, 16 rows 24.3 us against 22.6), in as even a number
-// of tiles as it goes, in whole runs of 8 (the XCDs) per group of rows
+// One workgroup per CU, the tiles in equal rounds, workgroups in whole runs of 8 (the XCDs) per group of rows.  Two workgroups per CU,
+// where registers allow it, bring nothing: 16 rows, 28672 x 4096 24.3 us against 22.6; 128 rows, 6144 x 1024 8.6 against 7.4.
 template <int NWAVE, int KW, int PF, int MT, bool WIDE, bool EXACT>
 void launch_rows(const Args &a) {
     const int groups = (a.M + 16 * MT - 1) / (16 * MT);
-    // every CU a workgroup (two of those that would fit bring nothing), an eighth of them to each XCD; the tiles in equal rounds
     const int most = groups <= 32 ? 256 / groups / 8 * 8 : 8, rounds = (a.p.n_tiles + most - 1) / most;
     const unsigned grid = (unsigned)groups * (unsigned)(((a.p.n_tiles + rounds - 1) / rounds + 7) / 8 * 8);
     if (a.act)
