@@ -770,12 +770,16 @@ HA_FP8_E4M3 = 3
 
 
 class Fp8Weight(NamedTuple):
-    """A weight matrix [N, K] as `linear_fp8` reads it: e4m3 tiles and their scales (`pack_weight_fp8`)."""
+    """A weight matrix [N, K] as `linear_fp8` reads it: e4m3 tiles and their scales (`pack_weight_fp8`).  parts: the rows of matrices
+    that were packed apart and lie behind each other here, where one of them does not begin on a multiple of 128 rows (the product
+    of more than 16 rows takes one scale for several tiles of a block of 128 rows, counted from the first: such matrices are then
+    multiplied one by one); else empty."""
     tiles: torch.Tensor
     scales: torch.Tensor
     N: int
     K: int
     glu: bool
+    parts: Tuple[int, ...] = ()
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
@@ -912,11 +916,11 @@ def pack_weight_fp8(w: torch.Tensor, scales: Optional[torch.Tensor] = None, glu:
     return out
 
 
-LINEAR_FP8_UNSPLIT_ROWS = 16     # up to this many rows no workspace is needed
+LINEAR_FP8_UNSPLIT_ROWS = 16     # up to this many rows no workspace is needed, and every tile's own scales are read
 
 
 def linear_fp8_workspace_bytes(m: int, weight: Fp8Weight) -> int:
-    return load_library().ha_linear_fp8_workspace_bytes(m, weight.N, weight.K, int(weight.glu))
+    return max(load_library().ha_linear_fp8_workspace_bytes(m, n, weight.K, int(weight.glu)) for n in weight.parts or (weight.N,))
 
 
 def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: torch.Tensor, residual: Optional[torch.Tensor] = None,
@@ -924,7 +928,7 @@ def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: to
     """out [M, N] = rows in 8 bits (q, scales) . W^T (+ residual), or [M, N / 2] = silu(gate) * up with swiglu (weights packed with
     glu); out fp32, bf16 or fp16, rounded once.  residual may be out itself.  ws: scratch of `linear_fp8_workspace_bytes` bytes,
     taken from torch's allocator where it is needed and not given."""
-    tiles, tile_scales, n, k, glu = weight
+    tiles, tile_scales, n, k, glu, parts = weight
     dev = _same_device(q, scales, tiles, tile_scales, out, residual)
     m = q.shape[0]
     q_sm, s_sm = _fp8_rows_of(q, scales, m, k)
@@ -941,6 +945,14 @@ def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: to
         if swiglu:
             raise ValueError("SwiGLU takes no residual")
         r, r_sm = residual.data_ptr(), _rows_of(residual, "residual", m, n, out.dtype)
+    if parts and m > LINEAR_FP8_UNSPLIT_ROWS:
+        at = row = 0
+        for rows in parts:
+            count = (rows + 15) // 16 * ((k + 127) // 128)
+            part = Fp8Weight(tiles[2048 * at:2048 * (at + count)], tile_scales[2 * at:2 * (at + count)], rows, k, False)
+            linear_fp8(q, scales, part, out[:, row:row + rows], None if residual is None else residual[:, row:row + rows], ws=ws)
+            at, row = at + count, row + rows
+        return out
     lib = _lib or load_library()
     if ws is None and m > LINEAR_FP8_UNSPLIT_ROWS:
         nbytes = lib.ha_linear_fp8_workspace_bytes(m, n, k, 1 if swiglu else 0)

@@ -78,8 +78,10 @@ def _stacks(modules: Sequence[Fp8Linear]) -> bool:
 
 def stacked_weight(owner: nn.Module, name: str, modules: Sequence[Fp8Linear]) -> _ops.Fp8Weight:
     """The modules' weights as one matrix, rows behind each other, kept on `owner` under `name`.  Packed tiles are ordered by row, so
-    the modules' own buffers become parts of the stacked ones: nothing is held twice.  Rebuilt when a module's buffer is no longer
-    that part (a move to another device, a loaded state dict): call it once before a graph is captured."""
+    the modules' own buffers become parts of the stacked ones: nothing is held twice.  Each module's blocks of 128 rows begin at its
+    own first row; where that is no multiple of 128 in the stacked matrix, the weight names its parts (`_ops.Fp8Weight`).  Rebuilt
+    when a module's buffer is no longer that part (a move to another device, a loaded state dict): call it once before a graph is
+    captured."""
     weight = owner.__dict__.get(name)
     if weight is not None and _parts_of(weight, modules):
         return weight
@@ -93,7 +95,9 @@ def stacked_weight(owner: nn.Module, name: str, modules: Sequence[Fp8Linear]) ->
         n, ns = m.tiles.numel(), m.tile_scales.numel()
         m.tiles, m.tile_scales = tiles[at:at + n], scales[s_at:s_at + ns]
         at, s_at = at + n, s_at + ns
-    weight = _ops.Fp8Weight(tiles, scales, sum(m.out_features for m in modules), modules[0].in_features, False)
+    rows = tuple(m.out_features for m in modules)
+    weight = _ops.Fp8Weight(tiles, scales, sum(rows), modules[0].in_features, False,
+                            rows if any(n % _ops.FP8_BLOCK for n in rows[:-1]) else ())
     owner.__dict__[name] = weight
     return weight
 

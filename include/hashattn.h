@@ -525,6 +525,9 @@ int ha_linear_tiled(const void *x, int64_t x_stride_m, const void *tiles, const 
  *                                   [ceil(N / 128), ceil(K / 128)]: taken over as they are.  glu = 1: w is [F gate rows; F up
  *                                   rows] (N = 2 F), each matrix with blocks of its own: w_scales then holds gate's rows of
  *                                   ceil(F / 128) blocks, then up's
+ * Each scale of `tile_scales` belongs to a block of 128 rows counted from the matrix's first (glu: of gate's and of up's), and
+ * ha_linear_fp8 takes one for all tiles of a block: packed matrices put behind each other are one packed matrix only where all but the
+ * last have a multiple of 128 rows.
  *
  * ha_linear_fp8: out [M, N] = x . W^T (+ residual [M, N] of out_dtype), or with act = HA_ACT_SWIGLU (weights packed with glu = 1)
  * out [M, N / 2] = silu(gate) * up.  Products exact, sums in fp32, ONE rounding to out_dtype at the end (residual and SwiGLU before
