@@ -12,6 +12,7 @@ embeddings and the lm_head stay as they are.  A converted layer's single-token s
 """
 from __future__ import annotations
 
+import warnings
 from typing import Optional, Sequence
 
 import torch
@@ -116,29 +117,41 @@ def _parts_of(weight: _ops.Fp8Weight, modules: Sequence[Fp8Linear]) -> bool:
 _ATTENTION, _MLP = ("q_proj", "k_proj", "v_proj", "o_proj"), ("gate_proj", "up_proj", "down_proj")
 
 
-def _is_layer(module: nn.Module) -> bool:
-    attn, mlp = getattr(module, "self_attn", None), getattr(module, "mlp", None)
-    return attn is not None and mlp is not None and all(isinstance(getattr(attn, n, None), nn.Linear) for n in _ATTENTION) \
-        and all(isinstance(getattr(mlp, n, None), nn.Linear) for n in _MLP)
+def _is_plain(lin) -> bool:
+    """Whether a projection computes x W^T (+ bias) and nothing else: no subclass (an adapter, a parametrization), no hook, no forward of
+    its own.  accelerate's placement of a model spread over devices only moves inputs, which the layer's own hook does too."""
+    if type(lin) is not nn.Linear or lin._forward_hooks or lin._forward_pre_hooks:
+        return False
+    return "forward" not in lin.__dict__ or type(getattr(lin, "_hf_hook", None)).__name__ == "AlignDevicesHook"
+
+
+def _projections(layer: nn.Module) -> list:
+    """The (owner, name) of a decoder layer's seven projections, and of the four of the module a converted attention module prefills
+    through, which holds weights of its own; empty if the module is no such layer."""
+    attn, mlp = getattr(layer, "self_attn", None), getattr(layer, "mlp", None)
+    found = [(attn, n) for n in _ATTENTION] + [(mlp, n) for n in _MLP]
+    if attn is None or mlp is None or not all(isinstance(getattr(o, n, None), nn.Linear) for o, n in found):
+        return []
+    twin = getattr(getattr(attn, "flash_forward", None), "__self__", None)
+    return found + [(twin, n) for n in _ATTENTION if isinstance(getattr(twin, n, None), nn.Linear)]
 
 
 def convert_fp8(model: nn.Module) -> nn.Module:
     """Replace the seven projections of every decoder layer in place by `Fp8Linear`.  The model is on the GPU; `convert_usa`, where it
-    is used, comes first (it copies 16-bit weights)."""
-    layers = [m for m in model.modules() if _is_layer(m)]
-    if not layers:
-        raise ValueError("no decoder layer with q/k/v/o and gate/up/down projections of type nn.Linear in this model")
-    for layer in layers:
-        attn, mlp = layer.self_attn, layer.mlp
-        # a converted attention module prefills through the module it replaced, which holds weights of its own
-        twin = getattr(getattr(attn, "flash_forward", None), "__self__", None)
-        for name in _ATTENTION:
-            new = Fp8Linear.from_linear(getattr(attn, name))
-            setattr(attn, name, new)
-            if twin is not None and isinstance(getattr(twin, name, None), nn.Linear):
-                setattr(twin, name, new)
-        for name in _MLP:
-            setattr(mlp, name, Fp8Linear.from_linear(getattr(mlp, name)))
+    is used, comes first (it copies 16-bit weights).  A layer with a projection that is more than an nn.Linear - a subclass with a
+    forward of its own, a hook - is left as it is, with a warning."""
+    layers = {m: p for m in model.modules() if (p := _projections(m))}
+    plain = {m: p for m, p in layers.items() if all(_is_plain(getattr(o, n)) for o, n in p)}
+    if not plain:
+        raise ValueError("no decoder layer with q/k/v/o and gate/up/down projections of type nn.Linear, without hooks, in this model")
+    if len(plain) < len(layers):
+        warnings.warn(f"{len(layers) - len(plain)} decoder layer(s) keep their projections: subclasses of nn.Linear, hooks or a forward of their own")
+    for layer, projections in plain.items():
+        attn = layer.self_attn
+        for owner, name in projections[:7]:
+            setattr(owner, name, Fp8Linear.from_linear(getattr(owner, name)))
+        for owner, name in projections[7:]:
+            setattr(owner, name, getattr(attn, name))
         for copy in ("_qkv_fused", "_qkv_tiles", "_o_tiles", "_gate_up_fused", "_gate_up_tiles", "_down_tiles"):
             attn.__dict__.pop(copy, None)        # stacked and tiled copies of the 16-bit weights, if steps ran before
     return model
