@@ -937,7 +937,7 @@ int ha_linear_fp8(const void *xq, int64_t xq_stride_m, const float *x_scales, in
     const Packed p = packed_shape(N, K, act);
     const int n_out = act ? N / 2 : N;
     HA_REQUIRE(xq_stride_m >= (int64_t)p.kb * HA_FP8_BLOCK && x_scales_stride_m >= p.kb && out_stride_m >= n_out &&
-                   (!residual || residual_stride_m >= N),
+                   (!residual || residual_stride_m == 0 || residual_stride_m >= N),
                HA_ERR_BAD_SHAPE, "strides smaller than the rows they span");
     const int es = ha_dtype_bytes(out_dtype);
     HA_REQUIRE(ha_aligned(xq, 16) && xq_stride_m % 16 == 0 && ha_aligned(tiles, 16), HA_ERR_MISALIGNED,

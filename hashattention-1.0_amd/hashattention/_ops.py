@@ -926,7 +926,7 @@ def linear_fp8_workspace_bytes(m: int, weight: Fp8Weight) -> int:
 def linear_fp8(q: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: torch.Tensor, residual: Optional[torch.Tensor] = None,
                swiglu: bool = False, ws: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out [M, N] = rows in 8 bits (q, scales) . W^T (+ residual), or [M, N / 2] = silu(gate) * up with swiglu (weights packed with
-    glu); out fp32, bf16 or fp16, rounded once.  residual may be out itself.  ws: scratch of `linear_fp8_workspace_bytes` bytes,
+    glu); out fp32, bf16 or fp16, rounded once.  residual may be out itself, or one row expanded to all (a bias).  ws: scratch of `linear_fp8_workspace_bytes` bytes,
     taken from torch's allocator where it is needed and not given."""
     tiles, tile_scales, n, k, glu, parts = weight
     dev = _same_device(q, scales, tiles, tile_scales, out, residual)

@@ -34,7 +34,7 @@ class Fp8Linear(nn.Module):
         self.in_features, self.out_features = weight.K, weight.N
         self.register_buffer("tiles", weight.tiles)
         self.register_buffer("tile_scales", weight.scales)
-        self.register_buffer("bias", None if bias is None else bias.detach())
+        self.register_buffer("bias", None if bias is None else bias.detach().contiguous())
 
     @classmethod
     def from_linear(cls, linear: nn.Linear) -> "Fp8Linear":
@@ -62,10 +62,14 @@ class Fp8Linear(nn.Module):
             rows = rows.contiguous()
         q, scales = _ops.fp8_rows(rows.shape[0], self.in_features, x.device)
         _ops.quantize_rows_fp8(rows, q, scales)
-        out = torch.empty(rows.shape[0], self.out_features, dtype=x.dtype, device=x.device)
-        _ops.linear_fp8(q, scales, self.packed, out)
-        if self.bias is not None:
-            out += self.bias
+        bias, dtype = self.bias, x.dtype
+        # the bias is added in front of the result's one rounding; one of another type that x's does not hold, to sums in fp32
+        if bias is not None and torch.promote_types(bias.dtype, dtype) != dtype:
+            dtype = torch.float32
+        out = torch.empty(rows.shape[0], self.out_features, dtype=dtype, device=x.device)
+        _ops.linear_fp8(q, scales, self.packed, out, None if bias is None else bias.to(dtype).expand(out.shape))
+        if dtype != x.dtype:
+            out = out.to(x.dtype)
         return out.view(*x.shape[:-1], self.out_features)
 
     def extra_repr(self) -> str:

@@ -529,7 +529,7 @@ int ha_linear_tiled(const void *x, int64_t x_stride_m, const void *tiles, const 
  * ha_linear_fp8 takes one for all tiles of a block: packed matrices put behind each other are one packed matrix only where all but the
  * last have a multiple of 128 rows.
  *
- * ha_linear_fp8: out [M, N] = x . W^T (+ residual [M, N] of out_dtype), or with act = HA_ACT_SWIGLU (weights packed with glu = 1)
+ * ha_linear_fp8: out [M, N] = x . W^T (+ residual [M, N] of out_dtype; a stride of 0 adds one row, a bias, to every row), or with act = HA_ACT_SWIGLU (weights packed with glu = 1)
  * out [M, N / 2] = silu(gate) * up.  Products exact, sums in fp32, ONE rounding to out_dtype at the end (residual and SwiGLU before
  * it).  16-bit results of more than 16 rows are summed by the 8-bit matrix instructions, which drop what lies more than 13 bits
  * below the largest of eight neighbouring products: about 1.5e-5 of the result, where the result's own rounding is 2^-9 or 2^-12 of
