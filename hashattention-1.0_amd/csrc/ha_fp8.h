@@ -50,16 +50,18 @@ __device__ __forceinline__ HaFp8Scale ha_fp8_scale(uint32_t top_bits, float comm
     return r;
 }
 
-// g / (1 + exp(-g)) to a relative 2^-21: exp(-g) as 2^t with the rounding error of t put back (2 ulp; 2^t alone loses |t| ulp), the
-// reciprocal to 1 ulp.  A quarter of the instructions of expf and an IEEE division, which bound the SwiGLU of a prompt (4096 x
-// 14336: 79 us, the memory's time is 60).  Far gates: exp(-g) overflows to infinity and the quotient is 0, or it vanishes and the
-// quotient is g; the correction is left out there (t itself may have overflowed, and its error is no number then).
+// g / (1 + exp(-g)) to a relative 2^-21 while exp(-g) is finite (g above -88.72): exp(-g) as 2^t with the rounding error of t put back
+// (2 ulp; 2^t alone loses |t| ulp), the reciprocal to 1 ulp.  A quarter of the instructions of expf and an IEEE division, which bound
+// the SwiGLU of a prompt (4096 x 14336: 79 us, the memory's time is 60).  Further out exp(-g) overflows to infinity and the quotient is 0,
+// or it vanishes and the quotient is g; the correction is left out there (t itself may have overflowed, and its error is no number
+// then).  Numerator and denominator are both taken at an eighth (powers of two: exact but for gates below 2^-123): the reciprocal of a
+// denominator above 2^126 would be subnormal, which the instruction does not give.
 __device__ __forceinline__ float ha_silu(float g) {
-    const float t = g * -1.44269504f;
-    const float lost = fmaf(g, -1.44269504f, -t) + g * -1.92596299e-8f;  // log2(e) is 1.44269504 + 1.926e-8
+    const float h = g * 0.125f, t = h * -11.5415603f;
+    const float lost = fmaf(h, -11.5415603f, -t) + h * -1.54077039e-7f;  // 8 log2(e) is 11.5415603 + 1.5408e-7
     float e = __builtin_amdgcn_exp2f(t);
-    if (fabsf(t) < 126.0f) e = fmaf(e, lost * 0.693147181f, e);
-    return g * __builtin_amdgcn_rcpf(1.0f + e);
+    if (fabsf(t) < 128.0f) e = fmaf(e, lost * 0.693147181f, e);
+    return h * __builtin_amdgcn_rcpf(fmaf(e, 0.125f, 0.125f));
 }
 
 #endif  // __HIPCC__
