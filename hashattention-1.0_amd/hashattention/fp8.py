@@ -44,13 +44,27 @@ class Fp8Linear(nn.Module):
     def packed(self) -> _ops.Fp8Weight:
         return _ops.Fp8Weight(self.tiles, self.tile_scales, self.out_features, self.in_features, False)
 
+    def __setattr__(self, name, value):
+        if name in ("tiles", "tile_scales"):
+            self._leave_stack()
+        super().__setattr__(name, value)
+
+    def _leave_stack(self):
+        """The stacked weight this module's buffers are parts of (`stacked_weight`) is held no longer: it is out of date."""
+        for holder in self.__dict__.pop("_stack", ()):
+            holder.clear()
+
     def _apply(self, fn, recurse=True):
         # casts (`model.bfloat16()`, `model.to(dtype)`) skip integers: the scales pass as their bits and stay fp32
-        self.tile_scales = self.tile_scales.view(torch.int32)
+        own = self._buffers
+        before = own["tiles"].data_ptr(), own["tile_scales"].data_ptr()
+        own["tile_scales"] = own["tile_scales"].view(torch.int32)
         try:
             return super()._apply(fn, recurse)
         finally:
-            self.tile_scales = self.tile_scales.view(torch.float32)
+            own["tile_scales"] = own["tile_scales"].view(torch.float32)
+            if before != (own["tiles"].data_ptr(), own["tile_scales"].data_ptr()):
+                self._leave_stack()
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-1:] != (self.in_features,):
@@ -87,9 +101,9 @@ def stacked_weight(owner: nn.Module, name: str, modules: Sequence[Fp8Linear]) ->
     own first row; where that is no multiple of 128 in the stacked matrix, the weight names its parts (`_ops.Fp8Weight`).  Rebuilt
     when a module's buffer is no longer that part (a move to another device, a loaded state dict): call it once before a graph is
     captured."""
-    weight = owner.__dict__.get(name)
-    if weight is not None and _parts_of(weight, modules):
-        return weight
+    holder = owner.__dict__.get(name)       # [weight], emptied by the first module whose buffers move on
+    if holder and _parts_of(holder[0], modules):
+        return holder[0]
     if not _stacks(modules):
         raise ValueError("rows of packed weights stack in whole tiles of 16")
     if modules[0].tiles.is_cuda and torch.cuda.is_current_stream_capturing():
@@ -103,7 +117,9 @@ def stacked_weight(owner: nn.Module, name: str, modules: Sequence[Fp8Linear]) ->
     rows = tuple(m.out_features for m in modules)
     weight = _ops.Fp8Weight(tiles, scales, sum(rows), modules[0].in_features, False,
                             rows if any(n % _ops.FP8_BLOCK for n in rows[:-1]) else ())
-    owner.__dict__[name] = weight
+    holder = owner.__dict__[name] = [weight]
+    for m in modules:
+        m.__dict__["_stack"] = (holder,)
     return weight
 
 
