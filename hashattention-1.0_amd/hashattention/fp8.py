@@ -17,6 +17,7 @@ from typing import Optional, Sequence
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _ops
 
@@ -69,7 +70,7 @@ class Fp8Linear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-1:] != (self.in_features,):
             raise ValueError(f"x has rows of {tuple(x.shape[-1:])}, the weight takes {self.in_features}")
-        if torch.is_grad_enabled() and x.requires_grad:
+        if torch.is_grad_enabled() and x.requires_grad or forward_ad.unpack_dual(x).tangent is not None:
             raise RuntimeError("Fp8Linear is for inference: no gradient flows through the 8-bit product (use torch.no_grad())")
         rows = x.reshape(-1, self.in_features)
         if self.in_features > 1 and rows.stride(1) != 1:
