@@ -22,7 +22,14 @@ import torch.nn.functional as F
 
 from . import _ops
 from .decode import HashDecodeLayer
+from .fp8 import Fp8Linear
 from .synthetic import UsaWeights, layer_dims
+
+
+def _refuse_converted(model) -> None:
+    if any(type(m) is Fp8Linear for m in model.modules()):
+        raise ValueError("the decoder copies 16-bit projections, which convert_fp8 has freed in this model: make the decoder first "
+                         "(fp8_projections=True for 8-bit projections), then convert the model")
 
 
 class LlamaShapedDecoder:
@@ -358,7 +365,9 @@ class LlamaShapedDecoder:
         layer): same weights, budgets from the model's config (`init_budget`, `heavy_budget`, `recent_budget`, as
         `convert_usa` reads them), caches for `batch` sequences of up to `cache_len` tokens; `fp8_projections`: the layers'
         projections in 8 bits.  Follow with
-        `prefill_from_hf` and `generate`."""
+        `prefill_from_hf` and `generate`.  A model that `convert_fp8` has converted holds no 16-bit projections any more and is
+        refused."""
+        _refuse_converted(model)
         cfg, usa0 = model.config, usa_modules[0]
         if usa0.rehash_every_step:
             raise NotImplementedError("the LSH baseline and CENTER re-hash the whole cache every step: use the patched layer")
@@ -413,6 +422,7 @@ class LlamaShapedDecoder:
 
     def load_hf_llama(self, model) -> None:
         """Copy the weights of a `transformers` LlamaForCausalLM of the same shape (used by the plumbing test)."""
+        _refuse_converted(model)
         sd = model.state_dict()
         self._gen_graph = self._gen_logits = None       # a captured generation step names the old weight buffers
         cast = lambda t: t.detach().to(self.device, self.dtype)
