@@ -824,9 +824,14 @@ def fp8_values(q: torch.Tensor, scales: torch.Tensor, k: int) -> torch.Tensor:
     return (q.float() * scales.repeat_interleave(FP8_BLOCK, dim=1))[:, :k]
 
 
+_INT_MAX = 2 ** 31 - 1          # sizes are C ints: ctypes passes the lowest 32 bits of a larger one without an error
+
+
 def _rows_of(t: torch.Tensor, what: str, m: int, k: int, dtype=None) -> int:
     """The row stride of t, checked to be [m, k] with contiguous rows of `dtype` (any floating type the kernels take, if None)."""
     s0, s1 = t.stride() if t.dim() == 2 else (0, 0)
+    if m > _INT_MAX or k > _INT_MAX:
+        raise ValueError(f"{what} [{m}, {k}]: rows and columns are counted in 32 bits")
     if t.shape != (m, k) or (s1 != 1 and k > 1):
         raise ValueError(f"{what} must be [{m}, {k}] with contiguous rows, got {tuple(t.shape)} with strides {t.stride()}")
     if t.dtype != dtype if dtype is not None else t.dtype not in _DTYPE:
@@ -893,6 +898,8 @@ def pack_weight_fp8(w: torch.Tensor, scales: Optional[torch.Tensor] = None, glu:
     if w.dim() != 2 or w.numel() == 0 or (w.stride(1) != 1 and w.shape[1] > 1):
         raise ValueError(f"w must be [N, K] with contiguous rows, got {tuple(w.shape)} with strides {w.stride()}")
     n, k = w.shape
+    if n > _INT_MAX or k > _INT_MAX:
+        raise ValueError(f"w [{n}, {k}]: rows and columns are counted in 32 bits")
     if glu and n % 2:
         raise ValueError(f"gate and up rows need an even number of weight rows, got {n}")
     if w.dtype == torch.float8_e4m3fn:
