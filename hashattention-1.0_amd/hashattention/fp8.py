@@ -109,12 +109,13 @@ def stacked_weight(owner: nn.Module, name: str, modules: Sequence[Fp8Linear]) ->
         raise ValueError("rows of packed weights stack in whole tiles of 16")
     if modules[0].tiles.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("the projections' weights are not stacked yet: run one step before capturing a graph")
-    tiles, scales = torch.cat([m.tiles for m in modules]), torch.cat([m.tile_scales for m in modules])
-    at = s_at = 0
-    for m in modules:
-        n, ns = m.tiles.numel(), m.tile_scales.numel()
-        m.tiles, m.tile_scales = tiles[at:at + n], scales[s_at:s_at + ns]
-        at, s_at = at + n, s_at + ns
+    with torch.inference_mode(False), torch.no_grad():      # ordinary tensors, which a state dict can be loaded into at any time
+        tiles, scales = torch.cat([m.tiles for m in modules]), torch.cat([m.tile_scales for m in modules])
+        at = s_at = 0
+        for m in modules:
+            n, ns = m.tiles.numel(), m.tile_scales.numel()
+            m.tiles, m.tile_scales = tiles[at:at + n], scales[s_at:s_at + ns]
+            at, s_at = at + n, s_at + ns
     rows = tuple(m.out_features for m in modules)
     weight = _ops.Fp8Weight(tiles, scales, sum(rows), modules[0].in_features, False,
                             rows if any(n % _ops.FP8_BLOCK for n in rows[:-1]) else ())
