@@ -605,6 +605,8 @@ class HeavyHitterMixin:
             return None
         if any(own[n].bias is not None for n in ("q_proj", "k_proj", "v_proj", "o_proj")) or not fp8 and self.q_proj.weight.dtype != torch.bfloat16:
             return None
+        if any(own[n]._forward_hooks or own[n]._forward_pre_hooks for n in ("q_proj", "k_proj", "v_proj", "o_proj")):
+            return None         # the step calls none of the four
         # a model spread over devices: its own hooks move the inputs
         if (self.q_proj.tiles if fp8 else self.q_proj.weight).device != hidden_states.device:
             return None
