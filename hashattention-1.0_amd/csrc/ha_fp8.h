@@ -61,7 +61,7 @@ __device__ __forceinline__ float ha_silu(float g) {
     const float lost = fmaf(h, -11.5415603f, -t) + h * -1.54077039e-7f;  // 8 log2(e) is 11.5415603 + 1.5408e-7
     float e = __builtin_amdgcn_exp2f(t);
     if (fabsf(t) < 128.0f) e = fmaf(e, lost * 0.693147181f, e);
-    return h * __builtin_amdgcn_rcpf(fmaf(e, 0.125f, 0.125f));
+    return h * __builtin_amdgcn_rcpf((1.0f + e) * 0.125f);
 }
 
 #endif  // __HIPCC__
