@@ -529,14 +529,16 @@ int ha_linear_tiled(const void *x, int64_t x_stride_m, const void *tiles, const 
  * ha_linear_fp8 takes one for all tiles of a block: packed matrices put behind each other are one packed matrix only where all but the
  * last have a multiple of 128 rows.
  *
- * ha_linear_fp8: out [M, N] = x . W^T (+ residual [M, N] of out_dtype; a stride of 0 adds one row, a bias, to every row), or with act = HA_ACT_SWIGLU (weights packed with glu = 1)
- * out [M, N / 2] = silu(gate) * up.  Products exact, sums in fp32, ONE rounding to out_dtype at the end (residual and SwiGLU before
- * it).  16-bit results of more than 16 rows are summed by the 8-bit matrix instructions, which drop what lies more than 13 bits
- * below the largest of eight neighbouring products: about 1.5e-5 of the result, where the result's own rounding is 2^-9 or 2^-12 of
- * it.  Where a matrix has too few tiles to fill the GPU, K is cut and the parts' sums go through the workspace, in two launches:
- * ha_linear_fp8_workspace_bytes(M, N, K, act) bytes, 16-byte aligned (0 for most sizes: NULL will do); calls that share one must
- * not overlap.  Any M, N, K; `residual` may be `out` itself.  Which kernel runs depends on the sizes, out_dtype and strides alone; a row's
- * outputs do not depend on the other rows' values.
+ * ha_linear_fp8: out [M, N] = x . W^T (+ residual [M, N] of out_dtype; a stride of 0 adds one row, a bias, to every row), or
+ * with act = HA_ACT_SWIGLU (weights packed with glu = 1) out [M, N / 2] = silu(gate) * up.  Products exact, sums in fp32, ONE
+ * rounding to out_dtype at the end (residual and SwiGLU before it).  16-bit results of more than 16 rows are summed by the
+ * 8-bit matrix instructions, which drop what lies more than 13 bits below the largest of eight neighbouring products: about
+ * 1.5e-5 of the result on normal numbers, 1e-4 where magnitudes spread widely, where the result's own rounding is 2^-9 (bf16)
+ * or 2^-12 (fp16) of it; where products cancel, up to 2^-10 of the sum of their magnitudes.  An fp32 out keeps its sums in fp32
+ * for any number of rows.  Where a matrix has too few tiles to fill the GPU, K is cut and the parts' sums go through the
+ * workspace, in two launches: ha_linear_fp8_workspace_bytes(M, N, K, act) bytes, 16-byte aligned (0 for most sizes: NULL will
+ * do); calls that share one must not overlap.  Any M, N, K; `residual` may be `out` itself.  Which kernel runs depends on the
+ * sizes, out_dtype and strides alone; a row's outputs do not depend on the other rows' values.
  */
 #define HA_FP8_BLOCK 128
 #define HA_FP8_E4M3 3 /* dtype code of ha_pack_weight_fp8 only */
